@@ -45,7 +45,7 @@ def listed():
         # one token through one projection
         dict(name="product_e4m3_1x2880x2880", kind="product", x="e4m3", rows=1, n=2880, k=2880, bias=True, out="f16"),
         # the ragged end of a prompt, an odd number of outputs
-        dict(name="product_e4m3_37x2049x2304", kind="product", x="e4m3", rows=37, n=2049, k=2304, bias=False, out="f32"),
+        dict(name="product_e4m3_37x2049x2304", kind="product", x="e4m3", rows=37, n=2049, k=2304, bias=False, out="bf16"),
         # a long chunk, 8-bit rows
         dict(name="product_e4m3_4096x4096x2880", kind="product", x="e4m3", rows=4096, n=4096, k=2880, bias=True, out="f16"),
         # a long chunk, both sides in 4 bits
@@ -78,7 +78,7 @@ def draw(rng):
         n, k = _log(rng, 16, 8192), _log(rng, 32, 8192, 32)
         rows = _log(rng, 1, min(8192, MOST_FLOPS // (2 * n * k)))
         return dict(kind=kind, x=rng.choice(["e4m3", "e4m3", "e2m1"]), rows=rows, n=n, k=k, bias=rng.random() < 0.5,
-                    out=rng.choice(["f16", "f16", "f32"]))
+                    out=rng.choice(["f16", "f16", "bf16"]))
     experts = rng.choice([8, 32, 64, 128, 256])
     d = _log(rng, 256, 4096, 64)
     f = min(_log(rng, 128, 4096, 64), max(64, MOST_WEIGHTS // experts // d // 64 * 64))
@@ -105,7 +105,7 @@ def work(case):
         return dict(bytes=moved + 2 * case["rows"] * _row_bytes("e4m3", case["d"]) + 2 * case["d"], flops=6 * n)
     if kind == "product":
         rows, n, k = case["rows"], case["n"], case["k"]
-        return dict(bytes=n * _row_bytes("e2m1", k) + rows * _row_bytes(case["x"], k) + rows * n * (4 if case["out"] == "f32" else 2),
+        return dict(bytes=n * _row_bytes("e2m1", k) + rows * _row_bytes(case["x"], k) + rows * n * 2,
                     flops=2 * rows * n * k)
     d, f, pairs = case["d"], case["f"], case["tokens"] * case["top_k"]
     used = case["experts"] * (1 - (1 - case["top_k"] / case["experts"]) ** case["tokens"])
