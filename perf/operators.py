@@ -21,7 +21,7 @@ own = False
 
 BLOCK = 32
 E4M3, E2M1 = 0, 1
-F16, BF16, F32 = 0, 1, 2
+BF16, F16, F32 = 0, 1, 2
 TYPES = {"f16": (F16, torch.float16), "bf16": (BF16, torch.bfloat16), "f32": (F32, torch.float32)}
 FORMATS = {"e4m3": E4M3, "e2m1": E2M1}
 GPTOSS = dict(d=2880, f=2880, experts=32, top_k=4, act="clamped", biases=True)   # gpt-oss-20B, whose experts are published in this format
