@@ -44,6 +44,11 @@ extern "C" {
 
 enum { SHRIKE_META_BF16 = 0, SHRIKE_META_F16 = 1 };
 enum { SHRIKE_ACT_GELU_TANH = 0, SHRIKE_ACT_SILU = 1, SHRIKE_ACT_CLAMPED_SWIGLU = 2 };
+/* Element types of the microscaled (MX) operators (the first two number as SHRIKE_META_* do), and their formats. */
+enum { SHRIKE_ELEM_BF16 = 0, SHRIKE_ELEM_F16 = 1, SHRIKE_ELEM_F32 = 2 };
+enum { SHRIKE_MX_E4M3 = 0, SHRIKE_MX_E2M1 = 1 };
+#define SHRIKE_MX_BLOCK 32u
+#define SHRIKE_MX_MAX_K 65536u
 enum { SHRIKE_RESIDENCY_EMPTY = 0, SHRIKE_RESIDENCY_LOADING = 1, SHRIKE_RESIDENCY_RESIDENT = 2 };
 
 const char *shrike_hip_last_error(void);
@@ -536,6 +541,70 @@ int shrike_hip_residual_add_f16(void *stream, void *d_hidden, const void *d_delt
 int shrike_hip_residual_add_rmsnorm_bf16w(void *stream, void *d_hidden, const void *d_delta,
                                           const void *d_weight, void *d_out, uint32_t d, float eps,
                                           uint32_t rows);
+
+/* ------------------------------------------- operators over microscaled (MX) blocks
+ * NO COUNTERPART IN THE REFERENCE, whose weights are group-affine. gpt-oss publishes its experts in this format; here they need
+ * not be quantised a second time, and the rows that meet them are 8 bits wide, on the scaled matrix instructions of gfx950.
+ *
+ * A block is SHRIKE_MX_BLOCK elements along a row that share one E8M0 scale byte s: 2^(s - 127), 255 = NaN. Elements are E4M3
+ * (one byte; no infinities, 0x7f and 0xff are NaN) or E2M1 (4 bits, two a byte, element 2k in the low half of byte k). A matrix of
+ * `rows` rows of `d` elements is codes[rows][d] (E4M3) or [rows][d / 2] (E2M1), 16-byte aligned, and scales[rows][d / 32], at any
+ * address, both without gaps; d is a multiple of 32.
+ * Quantising a block: s = max(0, e - 8) (E4M3) or max(0, e - 2) (E2M1), e the exponent field of the block's largest magnitude as
+ * an fp32; an element's code is the nearest of x * 2^(127 - s), ties to even, and what lies past the format's largest value (448, 6)
+ * becomes that. A block with an infinity or a NaN in it has s = 255 and zero codes: all of it reads as NaN. */
+
+/* Rows of fp16, bf16 or fp32 (`src_dtype`, SHRIKE_ELEM_*), src_stride_elements apart, into MX blocks. The source may start at any
+ * element; from 16-byte aligned rows it is read 16 bytes at a time. */
+int shrike_hip_mx_quantize(void *stream, const void *d_src, uint32_t src_dtype, uint64_t src_stride_elements, uint32_t format,
+                           void *d_codes, void *d_scales, uint64_t rows, uint32_t d);
+/* The values that MX blocks stand for, rounded to the output's type once; what lies between the rows is left as it is. */
+int shrike_hip_mx_dequantize(void *stream, const void *d_codes, const void *d_scales, uint32_t format, void *d_out, uint32_t out_dtype,
+                             uint64_t out_stride_elements, uint64_t rows, uint32_t d);
+
+/* shrike_hip_residual_add_rmsnorm_bf16w with its rows in 8 bits: sum = fp16(hidden + delta), out = fp16(norm(sum) * weight), the bits
+ * of that call, and codes, scales = the E4M3 blocks of `out`. d_sum may be d_hidden (in place); d_delta and d_sum are bound together
+ * or both NULL (no add). d_out may be NULL (the router reads fp16 rows, the experts the codes). d: a multiple of 32 up to
+ * SHRIKE_MAX_HIDDEN; buffers but d_scales 16-byte aligned. */
+int shrike_hip_residual_add_rmsnorm_bf16w_mx8(void *stream, const void *d_hidden, const void *d_delta, const void *d_weight, void *d_sum,
+                                              void *d_out, void *d_codes, void *d_scales, uint32_t d, float eps, uint32_t rows);
+
+/* out[r, i] = sum over k of x[r, k] * w[i, k], + bias[i] (bf16[n], may be NULL): x rows of MX blocks in either format, w rows of E2M1
+ * blocks; out fp16 or bf16, rows out_stride_elements apart (what lies between them is left as it is). The sum is fp32; within it the
+ * matrix instruction adds eight neighbouring products of E4M3 rows at a time and cuts off what lies below 2^-13 of the largest of
+ * them, so a result is good to the 16 bits it is returned in where its products do not cancel by more. k: a multiple of 32 up to
+ * SHRIKE_MX_MAX_K; n up to 2^24; rows up to 2^22. */
+int shrike_hip_mx_product(void *stream, const void *d_x_codes, const void *d_x_scales, uint32_t x_format, const void *d_w_codes,
+                          const void *d_w_scales, const void *d_bias, void *d_out, uint32_t out_dtype, uint64_t out_stride_elements,
+                          uint32_t rows, uint32_t n, uint32_t k);
+
+/* An expert's blob of E2M1 projections: gate codes, gate scales, up codes, up scales, down codes, down scales, and the bf16 biases
+ * of gate, up and down when asked for, one behind the other. The offsets of affine biases (`*_b_off`) are zero. d and f: multiples
+ * of 64. Returns the blob's size, 0 on invalid arguments. */
+uint64_t shrike_mx_expert_offsets_make(uint32_t d, uint32_t f, int additive_biases, shrike_expert_offsets *out);
+
+/* shrike_hip_prefill_grouped_ffn over such experts and 8-bit rows: route_partials[(token * top_k + rank) * d ..] =
+ * fp16(down . E4M3(glu(gate . x, up . x))) for every pair of a resident expert, where E4M3(.) quantises a row's activations to MX
+ * blocks from fp32. x: codes[query_count][d] and scales, as shrike_hip_residual_add_rmsnorm_bf16w_mx8 leaves them. The handle
+ * gives the shape, the activation and whether the experts have (bf16) biases; its weight bits play no part. Routes, pool, absent
+ * experts and max_row_tiles as there; the workspace holds the activations: 256-byte aligned, at least
+ * shrike_hip_mx_ffn_workspace_bytes(max_row_tiles, f). A pair's row depends on its token and its expert alone. */
+size_t shrike_hip_mx_ffn_workspace_bytes(uint32_t max_row_tiles, uint32_t f);
+int shrike_hip_mx_grouped_ffn(shrike_hip_moe *moe, void *stream, const shrike_pool_bases *pool, uint64_t pool_slot_stride,
+                              const shrike_expert_offsets *offsets, const shrike_hip_grouped_routes *routes, uint32_t max_row_tiles,
+                              const void *d_x_codes, const void *d_x_scales, void *d_route_partials, void *d_workspace, size_t workspace_bytes,
+                              uint32_t query_count, uint32_t d, uint32_t f, uint32_t top_k);
+
+/* shrike_hip_moe_phase1_batch and _phase2_batch in one call over such experts, for several sequences that decode one token each:
+ * y[t] = fp16(residual[t] + sum over k of weight[t, k] * (down_k . E4M3(glu(gate_k . x_t, up_k . x_t)))), hidden[t] = fp16(hidden[t] +
+ * y[t]). d_resolved_slots: u32[tokens, top_k], the experts' cells, SHRIKE_SLOT_SENTINEL a position that contributes nothing;
+ * d_routing_weights: fp16[tokens, top_k]; residual (NULL = 0), y and hidden (may be NULL): fp16[tokens, d]. The workspace holds the
+ * activations: 256-byte aligned, at least shrike_hip_mx_decode_workspace_bytes(). Up to 8,191 tokens. */
+size_t shrike_hip_mx_decode_workspace_bytes(uint32_t tokens, uint32_t top_k, uint32_t f);
+int shrike_hip_mx_decode_ffn(shrike_hip_moe *moe, void *stream, const shrike_pool_bases *pool, uint64_t pool_slot_stride,
+                             const uint32_t *d_resolved_slots, const shrike_expert_offsets *offsets, const void *d_x_codes,
+                             const void *d_x_scales, const void *d_routing_weights, const void *d_residual, void *d_y, void *d_hidden,
+                             void *d_workspace, size_t workspace_bytes, uint32_t d, uint32_t f, uint32_t top_k, uint32_t tokens);
 
 /* ----------------------------------------------------------------- plumbing
  * Device memory, streams, events and graphs for hosts without a HIP binding of

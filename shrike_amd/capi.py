@@ -18,6 +18,9 @@ SENTINEL = 0xFFFFFFFF
 POOL_PAGE = 16384
 META_BF16, META_F16 = 0, 1
 ACT_GELU_TANH, ACT_SILU, ACT_CLAMPED_SWIGLU = 0, 1, 2
+ELEM_BF16, ELEM_F16, ELEM_F32 = 0, 1, 2
+MX_E4M3, MX_E2M1 = 0, 1
+MX_BLOCK, MX_MAX_K = 32, 65536
 EMPTY, LOADING, RESIDENT = 0, 1, 2
 
 
@@ -330,6 +333,18 @@ SIGNATURES = {
     "shrike_hip_moe_decode_layer_launches": (C.c_int, [_VP, _VP, C.POINTER(DecodeLayerArgs), _U32]),
     "shrike_hip_moe_decode_layer_noalloc": (C.c_int, [C.POINTER(MoEDesc), _VP, C.POINTER(DecodeLayerArgs)]),
     "shrike_hip_residual_add_rmsnorm_bf16w": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _U32, C.c_float, _U32]),
+    # operators over microscaled blocks
+    "shrike_hip_mx_quantize": (C.c_int, [_VP, _VP, _U32, _U64, _U32, _VP, _VP, _U64, _U32]),
+    "shrike_hip_mx_dequantize": (C.c_int, [_VP, _VP, _VP, _U32, _VP, _U32, _U64, _U64, _U32]),
+    "shrike_hip_residual_add_rmsnorm_bf16w_mx8": (C.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _U32, C.c_float, _U32]),
+    "shrike_hip_mx_product": (C.c_int, [_VP, _VP, _VP, _U32, _VP, _VP, _VP, _VP, _U32, _U64, _U32, _U32, _U32]),
+    "shrike_mx_expert_offsets_make": (_U64, [_U32, _U32, C.c_int, C.POINTER(ExpertOffsets)]),
+    "shrike_hip_mx_ffn_workspace_bytes": (C.c_size_t, [_U32, _U32]),
+    "shrike_hip_mx_grouped_ffn": (C.c_int, [_VP, _VP, C.POINTER(PoolBases), _U64, C.POINTER(ExpertOffsets), C.POINTER(HipGroupedRoutes),
+                                            _U32, _VP, _VP, _VP, _VP, C.c_size_t, _U32, _U32, _U32, _U32]),
+    "shrike_hip_mx_decode_workspace_bytes": (C.c_size_t, [_U32, _U32, _U32]),
+    "shrike_hip_mx_decode_ffn": (C.c_int, [_VP, _VP, C.POINTER(PoolBases), _U64, _VP, C.POINTER(ExpertOffsets), _VP, _VP, _VP, _VP, _VP,
+                                           _VP, _VP, C.c_size_t, _U32, _U32, _U32, _U32]),
     "shrike_hip_malloc": (_VP, [_U64]),
     "shrike_hip_free": (C.c_int, [_VP]),
     "shrike_hip_host_alloc": (_VP, [_U64]),

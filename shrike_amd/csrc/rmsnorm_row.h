@@ -11,12 +11,12 @@ namespace shrike {
 // inv = 1 / sqrt(mean(h^2) + eps). The sum of squares is fp32: thread t takes the 8-element chunks
 // t, t+256, ... in one fma chain, a wave folds with the xor butterfly 32...1, the four wave sums are
 // added in order; what follows the sum is taken in fp64 and rounded to fp32 once, so the row is
-// reproducible bit for bit on a CPU. WRITE_HIDDEN stores h back over hidden. The normalised row goes
-// to out_row (global, may be null) and to out_lds (may be null; a barrier follows, so every thread
-// may read all of it on return). Every thread of the workgroup must call this.
-template <bool WRITE_HIDDEN>
-__device__ __forceinline__ void rmsnorm_row(uint16_t *hidden_row, const uint16_t *delta_row, const uint16_t *weight,
-                                            uint16_t *out_row, uint4 *out_lds, uint32_t d, float eps, float (&s_partial)[4]) {
+// reproducible bit for bit on a CPU. With a delta, h goes to sum_row (may be null, may be hidden_row); the
+// normalised row goes to sink(c, eight fp16 values) chunk by chunk, in the thread that owns the chunk.
+// Every thread of the workgroup must call this.
+template <typename Sink>
+__device__ __forceinline__ void rmsnorm_row_each(const uint16_t *hidden_row, const uint16_t *delta_row, uint16_t *sum_row, const uint16_t *weight,
+                                                 uint32_t d, float eps, float (&s_partial)[4], Sink sink) {
     const uint32_t chunks = d / 8u;  // d is a multiple of 8
     constexpr int kMine = SHRIKE_MAX_HIDDEN / 8 / 256;  // chunks a thread can own
     uint4 mine[kMine];
@@ -37,7 +37,7 @@ __device__ __forceinline__ void rmsnorm_row(uint16_t *hidden_row, const uint16_t
                 hw[j] = uint32_t(lo) | uint32_t(hi) << 16;
             }
             h = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-            if (WRITE_HIDDEN) reinterpret_cast<uint4 *>(hidden_row)[c] = h;
+            if (sum_row) reinterpret_cast<uint4 *>(sum_row)[c] = h;
         }
         mine[r] = h;
 #pragma unroll
@@ -67,10 +67,19 @@ __device__ __forceinline__ void rmsnorm_row(uint16_t *hidden_row, const uint16_t
             const float hi = __fmul_rn(__fmul_rn(f16_to_f32(uint16_t(hw[j] >> 16)), inv), bf16_to_f32(uint16_t(ww[j] >> 16)));
             o[j] = uint32_t(f32_to_f16(lo)) | uint32_t(f32_to_f16(hi)) << 16;
         }
-        const uint4 ov = make_uint4(o[0], o[1], o[2], o[3]);
+        sink(c, make_uint4(o[0], o[1], o[2], o[3]));
+    }
+}
+
+// WRITE_HIDDEN stores h back over hidden. The normalised row goes to out_row (global, may be null) and to out_lds (may be null; a
+// barrier follows, so every thread may read all of it on return).
+template <bool WRITE_HIDDEN>
+__device__ __forceinline__ void rmsnorm_row(uint16_t *hidden_row, const uint16_t *delta_row, const uint16_t *weight,
+                                            uint16_t *out_row, uint4 *out_lds, uint32_t d, float eps, float (&s_partial)[4]) {
+    rmsnorm_row_each(hidden_row, delta_row, WRITE_HIDDEN ? hidden_row : nullptr, weight, d, eps, s_partial, [&](uint32_t c, uint4 ov) {
         if (out_row) reinterpret_cast<uint4 *>(out_row)[c] = ov;
         if (out_lds) out_lds[c] = ov;
-    }
+    });
     if (out_lds) __syncthreads();
 }
 

@@ -173,6 +173,15 @@ def expert_offsets(d: int, f: int, bits: int = 4, additive_biases: bool = False)
     return off, stride
 
 
+def mx_expert_offsets(d: int, f: int, additive_biases: bool = False):
+    """The offsets of an expert's blob of E2M1 projections, and its size."""
+    off = ExpertOffsets()
+    size = capi.load().shrike_mx_expert_offsets_make(d, f, int(additive_biases), C.byref(off))
+    if size == 0:
+        raise ShrikeError(capi.last_error())
+    return off, size
+
+
 class ExpertPool:
     """shrike_hip_pool: the HBM cell arena and residency table of one layer."""
 
@@ -403,6 +412,18 @@ class MoE:
               "shrike_hip_moe_decode_layer_launches")
 
 
+    def mx_decode_workspace_bytes(self, tokens: int) -> int:
+        return capi.load().shrike_hip_mx_decode_workspace_bytes(tokens, self.desc.top_k, self.desc.f)
+
+    def encode_mx_decode_ffn(self, pool: ExpertPool, resolved_slots, offsets, x_codes, x_scales, routing_weights, residual, y, hidden,
+                             workspace: DeviceBuffer, top_k, tokens):
+        """The routed experts' FFN over MX blocks for `tokens` sequences, one token each (shrike_hip_mx_decode_ffn)."""
+        check(capi.load().shrike_hip_mx_decode_ffn(
+            self.handle, self._s(), pool.bases, pool.stride, ptr(resolved_slots), C.byref(offsets), ptr(x_codes), ptr(x_scales),
+            ptr(routing_weights), ptr(residual), ptr(y), ptr(hidden), ptr(workspace), workspace.nbytes, self.desc.d, self.desc.f, top_k,
+            tokens), "shrike_hip_mx_decode_ffn")
+
+
 class GroupedRoutesDevice:
     """Device buffers of shrike_hip_grouped_routes for up to `pairs` pairs over `num_experts`."""
 
@@ -492,6 +513,17 @@ class Prefill:
             "shrike_hip_prefill_streamed_batched")
         return count.value
 
+    def mx_ffn_workspace_bytes(self, max_row_tiles):
+        return capi.load().shrike_hip_mx_ffn_workspace_bytes(max_row_tiles, self.moe.desc.f)
+
+    def encode_mx_grouped_expert_gemms(self, pool: ExpertPool, offsets, routes: GroupedRoutesDevice, x_codes, x_scales, route_partials,
+                                       workspace: DeviceBuffer, query_count, top_k, max_row_tiles=None):
+        """encode_grouped_expert_gemms over E2M1 experts and E4M3 rows (shrike_hip_mx_grouped_ffn)."""
+        check(capi.load().shrike_hip_mx_grouped_ffn(
+            self.moe.handle, self._s(), pool.bases, pool.stride, C.byref(offsets), C.byref(routes.c),
+            routes.max_row_tiles if max_row_tiles is None else max_row_tiles, ptr(x_codes), ptr(x_scales), ptr(route_partials),
+            ptr(workspace), workspace.nbytes, query_count, self.moe.desc.d, self.moe.desc.f, top_k), "shrike_hip_mx_grouped_ffn")
+
     def encode_shared_expert(self, gate, up, down, bits, hidden, hidden_stride_elements, h1, query_count, f_shared,
                              workspace: DeviceBuffer | None = None, scalar_gate=None):
         """The shared expert for every token of the chunk; returns the workspace it used."""
@@ -532,3 +564,34 @@ def residual_add_rmsnorm_bf16w(hidden, delta, weight, out, d: int, eps: float, r
     check(capi.load().shrike_hip_residual_add_rmsnorm_bf16w(stream.handle if stream else None, ptr(hidden), ptr(delta),
                                                             ptr(weight), ptr(out), d, eps, rows),
           "shrike_hip_residual_add_rmsnorm_bf16w")
+
+
+def residual_add_rmsnorm_bf16w_mx8(hidden, delta, weight, total, out, codes, scales, d: int, eps: float, rows: int = 1,
+                                   stream: Stream | None = None) -> None:
+    """The same norm with its rows in E4M3 blocks: total = hidden + delta (may be hidden itself; None with delta None), out = the
+    normalised fp16 rows (may be None), codes and scales their MX blocks."""
+    check(capi.load().shrike_hip_residual_add_rmsnorm_bf16w_mx8(stream.handle if stream else None, ptr(hidden), ptr(delta), ptr(weight),
+                                                                ptr(total), ptr(out), ptr(codes), ptr(scales), d, eps, rows),
+          "shrike_hip_residual_add_rmsnorm_bf16w_mx8")
+
+
+def mx_quantize(src, src_dtype: int, src_stride_elements: int, fmt: int, codes, scales, rows: int, d: int,
+                stream: Stream | None = None) -> None:
+    """Rows of capi.ELEM_* elements into MX blocks of format capi.MX_E4M3 or MX_E2M1."""
+    check(capi.load().shrike_hip_mx_quantize(stream.handle if stream else None, ptr(src), src_dtype, src_stride_elements, fmt, ptr(codes),
+                                             ptr(scales), rows, d), "shrike_hip_mx_quantize")
+
+
+def mx_dequantize(codes, scales, fmt: int, out, out_dtype: int, out_stride_elements: int, rows: int, d: int,
+                  stream: Stream | None = None) -> None:
+    """The values that MX blocks stand for, as rows of capi.ELEM_* elements."""
+    check(capi.load().shrike_hip_mx_dequantize(stream.handle if stream else None, ptr(codes), ptr(scales), fmt, ptr(out), out_dtype,
+                                               out_stride_elements, rows, d), "shrike_hip_mx_dequantize")
+
+
+def mx_product(x_codes, x_scales, x_format: int, w_codes, w_scales, bias, out, out_dtype: int, out_stride_elements: int, rows: int, n: int,
+               k: int, stream: Stream | None = None) -> None:
+    """out[rows, n] = x . w^T (+ bias): x MX blocks in either format, w E2M1 blocks, bias bf16 or None, out fp16 or bf16."""
+    check(capi.load().shrike_hip_mx_product(stream.handle if stream else None, ptr(x_codes), ptr(x_scales), x_format, ptr(w_codes),
+                                            ptr(w_scales), ptr(bias), ptr(out), out_dtype, out_stride_elements, rows, n, k),
+          "shrike_hip_mx_product")
