@@ -49,6 +49,7 @@ enum { SHRIKE_ELEM_BF16 = 0, SHRIKE_ELEM_F16 = 1, SHRIKE_ELEM_F32 = 2 };
 enum { SHRIKE_MX_E4M3 = 0, SHRIKE_MX_E2M1 = 1 };
 #define SHRIKE_MX_BLOCK 32u
 #define SHRIKE_MX_MAX_K 65536u
+#define SHRIKE_MX_MAX_DECODE_TOKENS 64u
 enum { SHRIKE_RESIDENCY_EMPTY = 0, SHRIKE_RESIDENCY_LOADING = 1, SHRIKE_RESIDENCY_RESIDENT = 2 };
 
 const char *shrike_hip_last_error(void);
@@ -599,7 +600,9 @@ int shrike_hip_mx_grouped_ffn(shrike_hip_moe *moe, void *stream, const shrike_po
  * y[t] = fp16(residual[t] + sum over k of weight[t, k] * (down_k . E4M3(glu(gate_k . x_t, up_k . x_t)))), hidden[t] = fp16(hidden[t] +
  * y[t]). d_resolved_slots: u32[tokens, top_k], the experts' cells, SHRIKE_SLOT_SENTINEL a position that contributes nothing;
  * d_routing_weights: fp16[tokens, top_k]; residual (NULL = 0), y and hidden (may be NULL): fp16[tokens, d]. The workspace holds the
- * activations: 256-byte aligned, at least shrike_hip_mx_decode_workspace_bytes(). Up to 8,191 tokens. */
+ * activations: 256-byte aligned, at least shrike_hip_mx_decode_workspace_bytes(). Up to SHRIKE_MX_MAX_DECODE_TOKENS tokens: an
+ * expert that several of them route to has its gate and up read once for every 16 of its pairs. (How many tokens a call has may change the
+ * order of the sums over k, and so a result's last bit.) */
 size_t shrike_hip_mx_decode_workspace_bytes(uint32_t tokens, uint32_t top_k, uint32_t f);
 int shrike_hip_mx_decode_ffn(shrike_hip_moe *moe, void *stream, const shrike_pool_bases *pool, uint64_t pool_slot_stride,
                              const uint32_t *d_resolved_slots, const shrike_expert_offsets *offsets, const void *d_x_codes,

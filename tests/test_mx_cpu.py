@@ -94,7 +94,7 @@ def experts(d=128, f=64, biases=False):
     (dict(moe=None), "NULL"), (dict(d=64), "differs"), (dict(f=128), "differs"), (dict(top_k=0), "topK"), (dict(top_k=9), "topK"), (dict(stride=24), "geometry"),
     (dict(cells=0), "geometry"), (dict(base=A + 8), "aligned"), (dict(gate_w_off=8), "multiples of 16"), (dict(up_w_off=1 << 20), "does not fit"),
     (dict(down_s_off=1 << 20), "does not fit"), (dict(x=None), "NULL"), (dict(xs=None), "NULL"), (dict(out=None), "NULL"), (dict(ws=None), "NULL"),
-    (dict(x=A + 4), "aligned"), (dict(out=A + 8), "aligned"), (dict(ws=A + 16), "256-byte"), (dict(bytes=100), "needed"), (dict(tokens=MAXU32), "many|needed"),
+    (dict(x=A + 4), "aligned"), (dict(out=A + 8), "aligned"), (dict(ws=A + 16), "256-byte"), (dict(bytes=100), "needed"), (dict(tokens=MAXU32), "many|needed|GiB"),
     (dict(gate_ab_off=1, biases=1), "even"), (dict(down_ab_off=1 << 20, biases=1), "do not fit")])
 @pytest.mark.parametrize("kind", ["grouped", "decode"])
 def test_experts_refuse(change, word, kind):
