@@ -57,7 +57,7 @@ __device__ __forceinline__ uint32_t max_xor32(uint32_t v) {
 }
 
 // The activation of four neighbouring gate and up sums in each of two tiles: one MX block of 32 over the four lanes l, l ^ 16, l ^ 32,
-// l ^ 48. The activation goes to eight bits from fp32, without a rounding to fp16 between. (fminf and fmaxf drop a NaN: it is put back.)
+// l ^ 48. The activation goes to eight bits from fp32, without a rounding to fp16 between. (The clamps drop a NaN: it is put back.)
 struct MxActBlock {
     uint32_t codes[2];  // of the lane's four values in either tile
     uint32_t scale;
@@ -69,7 +69,11 @@ __device__ __forceinline__ MxActBlock mx_activate(const f32x4 (&gate)[2], const 
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float g = gate[i / 4][i % 4], u = up[i / 4][i % 4];
-            v[i] = __builtin_isunordered(g, u) ? __uint_as_float(0x7fc00000u) : glu_rt_fast(g, u, decltype(kind)::value);
+            v[i] = glu_rt_fast(g, u, decltype(kind)::value);
+            if (decltype(kind)::value == SHRIKE_ACT_CLAMPED_SWIGLU) {
+                asm volatile("" : "+v"(v[i]));  // (or the compiler branches round the exponential, lane by lane)
+                v[i] = __builtin_isunordered(g, u) ? __uint_as_float(0x7fc00000u) : v[i];
+            }
             top = max(top, magnitude_bits(v[i]));
         }
     };
@@ -102,6 +106,12 @@ __device__ __forceinline__ f32x4 mx_bias4(const uint16_t *bias, uint32_t n, uint
             if (n + i < rows) v[i] = bf16_to_f32(bias[n + i]);
     }
     return v;
+}
+
+// the same where the four are there: experts' outputs are multiples of 64
+__device__ __forceinline__ f32x4 mx_bias4(const uint16_t *bias, uint32_t n) {
+    const u16x4_by2 b = *reinterpret_cast<const u16x4_by2 *>(bias + n);
+    return f32x4{bf16_to_f32(b[0]), bf16_to_f32(b[1]), bf16_to_f32(b[2]), bf16_to_f32(b[3])};
 }
 
 // Four outputs to the nearest of 16 bits. (Both conversions are made, two values an instruction, and one is taken: fewer cycles than a branch.)
@@ -401,8 +411,8 @@ __global__ __launch_bounds__(64 * WAVES, LEAST) void k_mx_few(MxArgs a) {
             gate[i] = PARTS > 1 ? total(i) : acc[0][i];
             up[i] = PARTS > 1 ? total(2u + i) : acc[0][2u + i];
             if (a.ebias) {
-                gate[i] += mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.gate_ab_off), n0 + 16u * i + 4u * q, a.n);
-                up[i] += mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.up_ab_off), n0 + 16u * i + 4u * q, a.n);
+                gate[i] += mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.gate_ab_off), n0 + 16u * i + 4u * q);
+                up[i] += mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.up_ab_off), n0 + 16u * i + 4u * q);
             }
         }
         const MxActBlock b = mx_activate(gate, up, a.act_kind);
@@ -431,7 +441,7 @@ __global__ __launch_bounds__(64 * WAVES, LEAST) void k_mx_few(MxArgs a) {
                 const uint32_t cell = a.slots[row];
                 if (cell == kSentinel) continue;
                 const uint8_t *at = cell_base(a.pool, cell, a.stride) + a.off.down_ab_off;
-                v += f16_to_f32(a.weights[row]) * mx_bias4(reinterpret_cast<const uint16_t *>(at), n, a.n);
+                v += f16_to_f32(a.weights[row]) * mx_bias4(reinterpret_cast<const uint16_t *>(at), n);
             }
         const size_t at = size_t(blockIdx.y) * a.n + n;
         uint32_t out[4], sum[4];
@@ -553,14 +563,17 @@ struct MxTile {
                 MxFragment<XF> f;
                 uint32_t scale;
             };
-            auto fetch = [&](int t) {
-                Rows r;
-                r.f.piece[0] = *reinterpret_cast<const u32x4 *>(rows + t * 2048u + 16u * ((half_x + q) ^ (m >> 1)));
-                if constexpr (XF == SHRIKE_MX_E4M3) r.f.piece[1] = *reinterpret_cast<const u32x4 *>(rows + t * 2048u + 16u * ((4u + q) ^ (m >> 1)));
-                r.scale = scale_x[t * 256u];
-                return r;
+            auto fetch = [&](Rows &r, int t, int part) {
+                if (part == 0) r.f.piece[0] = *reinterpret_cast<const u32x4 *>(rows + t * 2048u + 16u * ((half_x + q) ^ (m >> 1)));
+                if constexpr (XF == SHRIKE_MX_E4M3)
+                    if (part == 1) r.f.piece[1] = *reinterpret_cast<const u32x4 *>(rows + t * 2048u + 16u * ((4u + q) ^ (m >> 1)));
+                if (part == 2) r.scale = scale_x[t * 256u];
             };
-            Rows now = fetch(0), next = now;
+            Rows now, next;
+#pragma unroll
+            for (int part = 0; part < 3; ++part) fetch(now, 0, part);
+            next.f = now.f;
+            next.scale = now.scale;
             u32x4 wf[8];
             uint32_t ws[8];
 #pragma unroll
@@ -573,22 +586,20 @@ struct MxTile {
             }
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                if (t + 1 < MT) next = fetch(t + 1);
-                __builtin_amdgcn_sched_barrier(0);  // (asked for first: the compiler would put it where registers come free, too late)
+                // between the products, one thing each: the next rows' operands, then loads
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[t][i] = mx_multiply<XF>(wf[i], now.f, acc[t][i], ws[i], now.scale);
+                for (int i = 0; i < 8; ++i) {
+                    acc[t][i] = mx_multiply<XF>(wf[i], now.f, acc[t][i], ws[i], now.scale);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (t + 1 < MT && i < 3) fetch(next, t + 1, i);
+                    if (i >= 3) issue<NEXT_X, NEXT_W>(s, 5 * t + i - 3, load_x, load_w);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 // (the products stay ahead of what follows: they have no effect that would keep the compiler from moving them)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) asm volatile("" : "+a"(acc[t][i]));
-                if constexpr (NEXT_X)
-#pragma unroll
-                    for (int j = 4 * t; j < min(4 * t + 4, MT); ++j) load_x(s / kSteps + 1u, j);
-                if constexpr (NEXT_W)
-#pragma unroll
-                    for (int j = 8 * (4 * t - MT) / (3 * MT); j < 8 * (4 * (t + 1) - MT) / (3 * MT); ++j)
-                        if (j >= 0) load_w(s / 2u + 1u, j);
-                __builtin_amdgcn_sched_barrier(0);
-                now = next;
+                now.f = next.f;  // (one by one: with the structure's padding it would go through memory)
+                now.scale = next.scale;
             }
         };
 #pragma unroll
@@ -635,6 +646,18 @@ struct MxTile {
         }
         multiply(s, no, no, yes);
     }
+
+    // The load for place `at` of a step's 5 MT between products: the rows' first, one a place, then the weights', spread over what is left.
+    template <bool NEXT_X, bool NEXT_W, typename LoadX, typename LoadW>
+    static __device__ __forceinline__ void issue(uint32_t s, int at, LoadX load_x, LoadW load_w) {
+        constexpr int kPlaces = 5 * MT - MT;
+        if constexpr (NEXT_X)
+            if (at < MT) load_x(s / kSteps + 1u, at);
+        if constexpr (NEXT_W)
+            if (at >= MT)
+#pragma unroll
+                for (int j = 8 * (at - MT) / kPlaces; j < 8 * (at - MT + 1) / kPlaces; ++j) load_w(s / 2u + 1u, j);
+    }
 };
 
 template <int XF, int MT, MxWork WORK>
@@ -679,15 +702,16 @@ __device__ __forceinline__ void mx_tile(const MxArgs &a, uint8_t *lds, uint32_t 
         constexpr uint32_t kRoom = MT * 16u * 64u;
         wait_loads_and_sync<0>();
         uint8_t *room = lds + wave * kRoom;
+        if (first + wn * 64u >= a.n) return;  // (outputs are multiples of 64)
+        uint32_t scale[MT];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             const uint32_t f0 = first + wn * 64u + 32u * b;
-            if (f0 >= a.n) break;
             f32x4 bias[4] = {};
             if (a.ebias)
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i)
-                    bias[i] = mx_bias4(reinterpret_cast<const uint16_t *>(base + (i < 2u ? a.off.gate_ab_off : a.off.up_ab_off)), f0 + 16u * (i % 2u) + 4u * q, a.n);
+                    bias[i] = mx_bias4(reinterpret_cast<const uint16_t *>(base + (i < 2u ? a.off.gate_ab_off : a.off.up_ab_off)), f0 + 16u * (i % 2u) + 4u * q);
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const uint32_t r = r0 + 16u * t;
@@ -697,7 +721,8 @@ __device__ __forceinline__ void mx_tile(const MxArgs &a, uint8_t *lds, uint32_t 
                 uint32_t *to = reinterpret_cast<uint32_t *>(room + (16u * t + m) * 64u) + q;
                 to[4u * ((2u * b) ^ (m / 4u))] = q8.codes[0];
                 to[4u * ((2u * b + 1u) ^ (m / 4u))] = q8.codes[1];
-                if (q == 0 && r < rows) a.act_scales[size_t(row0 + r) * (a.n / kMxBlock) + f0 / kMxBlock] = uint8_t(q8.scale);
+                scale[t] = b == 0 ? q8.scale : scale[t] | q8.scale << 8;
+                if (b == 1 && q == 0 && r < rows) *reinterpret_cast<uint16_t *>(a.act_scales + size_t(row0 + r) * (a.n / kMxBlock) + f0 / kMxBlock - 1u) = uint16_t(scale[t]);
             }
         }
         const uint32_t f16 = first + wn * 64u + 16u * (lane % 4u);
@@ -712,9 +737,9 @@ __device__ __forceinline__ void mx_tile(const MxArgs &a, uint8_t *lds, uint32_t 
         f32x4 bias[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const uint16_t *from_bias = a.bias;
-            if constexpr (WORK == MxWork::kDown) from_bias = a.ebias ? reinterpret_cast<const uint16_t *>(base + a.off.down_ab_off) : nullptr;
-            bias[i] = mx_bias4(from_bias, n0 + 16u * i, a.n);
+            if constexpr (WORK == MxWork::kDense) bias[i] = mx_bias4(a.bias, n0 + 16u * i, a.n);
+            else if (a.ebias) bias[i] = mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.down_ab_off), min(n0 + 16u * i, a.n - 4u));
+            else bias[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         // Through LDS, where a wave has room for its own rows of 128 outputs: so that a store takes whole lines of four rows. (Straight from the
         // registers a line is four stores of a quarter of it each: 4,096 x 4,096 outputs 17 us in place of 7.) 16-byte pieces swapped as ever.
@@ -722,6 +747,14 @@ __device__ __forceinline__ void mx_tile(const MxArgs &a, uint8_t *lds, uint32_t 
         static_assert(4u * kRoom <= MxTileLds<MT>::kBytes);
         wait_loads_and_sync<0>();
         uint8_t *room = lds + wave * kRoom;
+        // down: where a lane's rows go, the wave's rows lane and lane + 64
+        uint32_t place[2] = {0, 0};
+        if constexpr (WORK == MxWork::kDown)
+#pragma unroll
+            for (uint32_t i = 0; i < (MT > 4 ? 2u : 1u); ++i) {
+                const shrike_token_expert_pair p = a.pairs[pair0 + min(wm * 16u * MT + 64u * i + lane, rows - 1u)];
+                place[i] = p.token * a.top_k + p.rank;
+            }
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -730,10 +763,11 @@ __device__ __forceinline__ void mx_tile(const MxArgs &a, uint8_t *lds, uint32_t 
                 *reinterpret_cast<uint2 *>(room + (16u * t + m) * 256u + 16u * ((2u * i + q / 2u) ^ m) + q % 2u * 8u) = h;
             }
         const uint32_t n8 = first + wn * 128u + 8u * m;
-#pragma unroll 4
+#pragma unroll
         for (uint32_t j = 0; j < 4u * MT; ++j) {
             const uint32_t r = 4u * j + q, at = wm * 16u * MT + r;
             const uint4 v = *reinterpret_cast<const uint4 *>(room + r * 256u + 16u * (m ^ (r & 15u)));
+            const uint32_t slot = uint32_t(__shfl(int(place[MT > 4 ? j / 16u : 0u]), int(r % 64u)));
             if (at >= rows || n8 >= a.n) continue;
             uint16_t *to;
             bool whole = true;
@@ -741,8 +775,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs &a, uint8_t *lds, uint32_t 
                 to = a.out + (row0 + at) * a.out_stride;
                 whole = a.out_whole && n8 + 8u <= a.n;
             } else {
-                const shrike_token_expert_pair p = a.pairs[pair0 + at];
-                to = a.out + (size_t(p.token) * a.top_k + p.rank) * a.n;
+                to = a.out + size_t(slot) * a.n;
             }
             if (whole) {
                 *reinterpret_cast<uint4 *>(to + n8) = v;
@@ -1006,8 +1039,8 @@ __device__ __forceinline__ void mx_thin(const MxArgs &a, uint8_t *lds, uint32_t 
             if (a.ebias)
 #pragma unroll
                 for (uint32_t i = 0; i < 2; ++i) {
-                    gate[i] += mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.gate_ab_off), f0 + 16u * i + 4u * q, a.n);
-                    up[i] += mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.up_ab_off), f0 + 16u * i + 4u * q, a.n);
+                    gate[i] += mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.gate_ab_off), f0 + 16u * i + 4u * q);
+                    up[i] += mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.up_ab_off), f0 + 16u * i + 4u * q);
                 }
             const MxActBlock q8 = mx_activate(gate, up, a.act_kind);
             const size_t to_row = which.out_row(row);
@@ -1018,19 +1051,21 @@ __device__ __forceinline__ void mx_thin(const MxArgs &a, uint8_t *lds, uint32_t 
                 if (q == 0) a.act_scales[to_row * (a.n / kMxBlock) + f0 / kMxBlock] = uint8_t(q8.scale);
             }
         } else {
+            if (first + wave * 64u >= a.n) return;
             // Through LDS, the rows' halves of 128 bytes, so that whole lines leave; a wave's own half of its weights, which it has read.
             uint8_t *stage = lds + place_of(c + kPlaces - 1u) + kX + wave * 8192u;
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 f32x4 v = acc[t][i];
-                if (a.ebias) v += mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.down_ab_off), first + wave * 64u + 16u * i + 4u * q, a.n);
+                if (a.ebias) v += mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.down_ab_off), first + wave * 64u + 16u * i + 4u * q);
                 *reinterpret_cast<uint2 *>(stage + row * 128u + 8u * ((4u * i + q) ^ (2u * (m & 7u)))) = mx_pack4(v, SHRIKE_ELEM_F16);
             }
 #pragma unroll
             for (uint32_t i = 0; i < 2; ++i) {
                 const uint32_t r = 16u * t + 8u * i + lane / 8u, n = first + wave * 64u + 8u * (lane % 8u);
+                const size_t to_row = which.out_row(r);
                 if (r >= rows || n >= a.n) continue;
-                *reinterpret_cast<u32x4 *>(a.out + which.out_row(r) * a.n + n) = *reinterpret_cast<const u32x4 *>(stage + r * 128u + 16u * ((lane % 8u) ^ (r & 7u)));
+                *reinterpret_cast<u32x4 *>(a.out + to_row * a.n + n) = *reinterpret_cast<const u32x4 *>(stage + r * 128u + 16u * ((lane % 8u) ^ (r & 7u)));
             }
         }
     }
@@ -1039,14 +1074,10 @@ __device__ __forceinline__ void mx_thin(const MxArgs &a, uint8_t *lds, uint32_t 
 // Rows of a chunk: gate and up take a pair's token's, and leave them in the table's order; down leaves them with the pair's token.
 template <MxWork WORK>
 struct MxChunkRows {
-    const MxArgs &a;
-    uint32_t row0, pair0;
-    __device__ __forceinline__ uint32_t x_row(uint32_t r) const { return WORK == MxWork::kGateUp ? a.pairs[pair0 + r].token : row0 + r; }
-    __device__ __forceinline__ size_t out_row(uint32_t r) const {
-        if constexpr (WORK == MxWork::kGateUp) return row0 + r;
-        const shrike_token_expert_pair p = a.pairs[pair0 + r];
-        return size_t(p.token) * a.top_k + p.rank;
-    }
+    uint32_t row0, there;  // `there`: of row `lane`, gate and up its token, down where it goes
+    __device__ __forceinline__ uint32_t of(uint32_t r) const { return uint32_t(__shfl(int(there), int(r))); }
+    __device__ __forceinline__ uint32_t x_row(uint32_t r) const { return WORK == MxWork::kGateUp ? of(r) : row0 + r; }
+    __device__ __forceinline__ size_t out_row(uint32_t r) const { return WORK == MxWork::kGateUp ? row0 + r : of(r); }
 };
 template <MxWork WORK>
 __global__ __launch_bounds__(128, 2) void k_mx_expert_thin(MxArgs a) {
@@ -1057,7 +1088,8 @@ __global__ __launch_bounds__(128, 2) void k_mx_expert_thin(MxArgs a) {
     if (tile.cell == kSentinel || tile.rows == 0) return;
     const uint8_t *base = cell_base_uniform(a.pool, tile.cell, a.stride);
     const uint32_t rows = min(uint32_t(__builtin_amdgcn_readfirstlane(int(tile.rows))), kRowTile), pair0 = uint32_t(__builtin_amdgcn_readfirstlane(int(tile.pair_start)));
-    const MxChunkRows<WORK> which = {a, number * kRowTile, pair0};
+    const shrike_token_expert_pair p = a.pairs[pair0 + min(threadIdx.x & 63u, rows - 1u)];
+    const MxChunkRows<WORK> which = {number * kRowTile, WORK == MxWork::kGateUp ? p.token : p.token * a.top_k + p.rank};
     if (rows > 32u) mx_thin<4, WORK>(a, lds, rows, which, base);
     else if (rows > 16u) mx_thin<2, WORK>(a, lds, rows, which, base);
     else mx_thin<1, WORK>(a, lds, rows, which, base);
