@@ -12,7 +12,7 @@
 // exact there. With N(0, 1) rows that is 5e-6 of the result, with rows of outliers a hundred times the rest 6e-5: under the outputs'
 // rounding to 16 bits (2^-11 and 2^-8 a half step), which is why no output is 32 bits wide. Sums over the steps are fp32 throughout.
 //
-// Three kernels. k_mx_few: up to 64 rows, weights read once, straight from memory into the operands' registers, k split over the waves.
+// Three kernels. k_mx_few: up to 64 rows a workgroup, weights read straight from memory into the operands' registers, k split over the waves.
 // mx_tile: 256 rows against 256 weight rows through LDS, four waves, bound by the matrix cores and LDS. mx_thin: up to 64 rows of an
 // expert against 128 weight rows, through LDS too, several workgroups a compute unit, bound by reading the weights.
 #include "decode_launch.h"
@@ -928,7 +928,7 @@ __device__ __forceinline__ void mx_thin(const MxArgs &a, uint8_t *lds, uint32_t 
         x_at[i] = start + 16u * (m ^ (r % 16u));
         x_end[i] = start + a.k - 16u;
     }
-    const uint8_t *const w0 = uniform(base), *const x0 = uniform(a.x);
+    const uint8_t *const w0 = uniform(base), *const x0 = uniform(a.x + size_t(which.x_row0()) * a.k);
     auto load = [&](uint32_t c) {
         const uint32_t place = lds0 + place_of(c);
 #pragma unroll
@@ -939,7 +939,7 @@ __device__ __forceinline__ void mx_thin(const MxArgs &a, uint8_t *lds, uint32_t 
     // The scales of three chunks, 8 a chunk: a weight row a lane, a row of x by one wave's 32. Where the row has fewer left, its last 8; a row that has not
     // as many is read byte by byte.
     const uint8_t *const w_scales = base + scales_of(lane) + weight_row(lane) * blocks;
-    const uint8_t *const x_scales = a.x_scales + size_t(x_row(MT <= 2 ? min(lane % 32u, 16u * MT - 1u) : lane)) * blocks;
+    const uint8_t *const x_scales = a.x_scales + size_t(which.x_row0() + x_row(MT <= 2 ? min(lane % 32u, 16u * MT - 1u) : lane)) * blocks;
     uint2 sw[3], sx[3];
     auto scales_from = [&](uint32_t c) { return blocks >= 8u ? min(8u * c, blocks - 8u) : 0u; };
     auto load_scales = [&](uint32_t c) {
@@ -1076,7 +1076,8 @@ template <MxWork WORK>
 struct MxChunkRows {
     uint32_t row0, there;  // `there`: of row `lane`, gate and up its token, down where it goes
     __device__ __forceinline__ uint32_t of(uint32_t r) const { return uint32_t(__shfl(int(there), int(r))); }
-    __device__ __forceinline__ uint32_t x_row(uint32_t r) const { return WORK == MxWork::kGateUp ? of(r) : row0 + r; }
+    __device__ __forceinline__ uint32_t x_row0() const { return WORK == MxWork::kGateUp ? 0u : row0; }  // (the activations may pass 4 GiB)
+    __device__ __forceinline__ uint32_t x_row(uint32_t r) const { return WORK == MxWork::kGateUp ? of(r) : r; }
     __device__ __forceinline__ size_t out_row(uint32_t r) const { return WORK == MxWork::kGateUp ? row0 + r : of(r); }
 };
 template <MxWork WORK>
@@ -1099,6 +1100,7 @@ __global__ __launch_bounds__(128, 2) void k_mx_expert_thin(MxArgs a) {
 struct MxPairRows {
     uint32_t pair, top_k;  // lane m of each 16: row m's
     __device__ __forceinline__ uint32_t of(uint32_t r) const { return uint32_t(__shfl(int(pair), int(r & 15u))); }
+    __device__ __forceinline__ uint32_t x_row0() const { return 0; }
     __device__ __forceinline__ uint32_t x_row(uint32_t r) const { return of(r) / top_k; }
     __device__ __forceinline__ size_t out_row(uint32_t r) const { return of(r); }
 };
@@ -1113,15 +1115,37 @@ __global__ __launch_bounds__(128, 2) void k_mx_decode_thin(MxArgs a) {
 
 constexpr uint32_t kMxExpertLds = MxTileLds<8>::kBytes;  // the widest instance's
 
+template <int XF, int MT>
+static void launch_tiles(const MxArgs &a, hipStream_t s) {
+    const uint32_t tiles = (a.n + 255u) / 256u * ((a.rows + 32u * MT - 1u) / (32u * MT));
+    hipLaunchKernelGGL((k_mx_product<XF, MT>), dim3((tiles + 7u) / 8u * 8u), dim3(256), MxTileLds<MT>::kBytes, s, a);
+}
+
+// By rows and by how many workgroups a shape would have. Measured, us, E4M3 | E2M1 rows:
+//                                  64 x 16 outputs, k over 8 waves   64 x 256    128 x 256   256 x 256
+//    65 rows of 2,880 x 2,880              11.4 |  7.7              15.7 | 13.7 22.5 | 18.1 35.8 | 25.8
+//   128                                    13.6 |  9.0              15.6 | 13.9 22.5 | 18.4 36.6 | 26.8
+//   128 rows of 4,096 x 2,304              14.4 |  8.5              13.1 | 11.6 19.1 | 15.7 30.9 | 23.2
+//   256 rows of 2,880 x 2,880              19.9 | 12.4              15.7 | 13.9 22.7 | 18.7 36.8 | 27.1
+//   256 rows of 4,096 x 2,304              26.8 | 14.9              13.4 | 12.0 19.3 | 16.2 30.9 | 23.6
+// 1,024 rows of 2,880 x 2,880              70.5 | 40.0              18.4 | 15.8 24.2 | 20.0 38.2 | 28.5
+// 1,536 (288 workgroups of 64 x 256)      101   | 54.8              36.7 | 33.6 25.1 | 21.0 38.7 | 29.2
+// 2,048                                   134   | 72.3              36.9 | 34.2 26.2 | 22.1 39.0 | 29.9
+// Few workgroups read the rows once each: 384 of them from E4M3's bytes, 768 from E2M1's, are where that costs as much as the tiles' start.
+// Of the tiles the lowest that are dealt out in one go: a compute unit takes one at a time.
 template <int XF>
 static int launch_product(const MxArgs &a, hipStream_t s) {
-    if (a.rows <= 16u) {
+    const uint64_t columns = (a.n + 255u) / 256u, few = uint64_t((a.n + 15u) / 16u) * ((a.rows + 63u) / 64u);
+    if (a.rows <= 16u)
         hipLaunchKernelGGL((k_mx_few<XF, 1, 1, 8, 8, 4, MxWork::kDense>), dim3((a.n + 15u) / 16u, 1), dim3(512), 0, s, a);
-    } else if (a.rows <= 64u) {
-        hipLaunchKernelGGL((k_mx_few<XF, 4, 1, 8, 8, 2, MxWork::kDense>), dim3((a.n + 15u) / 16u, 1), dim3(512), 0, s, a);
-    } else {
-        hipLaunchKernelGGL((k_mx_product<XF, 8>), dim3(((a.n + 255u) / 256u * ((a.rows + 255u) / 256u) + 7u) / 8u * 8u), dim3(256), MxTileLds<8>::kBytes, s, a);
-    }
+    else if (a.rows <= 64u || few <= (XF == SHRIKE_MX_E4M3 ? 384u : 768u))
+        hipLaunchKernelGGL((k_mx_few<XF, 4, 1, 8, 8, 2, MxWork::kDense>), dim3((a.n + 15u) / 16u, (a.rows + 63u) / 64u), dim3(512), 0, s, a);
+    else if (columns * ((a.rows + 63u) / 64u) <= 256u)
+        launch_tiles<XF, 2>(a, s);
+    else if (columns * ((a.rows + 127u) / 128u) <= 256u)
+        launch_tiles<XF, 4>(a, s);
+    else
+        launch_tiles<XF, 8>(a, s);
     SHRIKE_HIP(hipGetLastError());
     return 0;
 }
@@ -1237,7 +1261,8 @@ int shrike_hip_mx_grouped_ffn(shrike_hip_moe *moe, void *stream, const shrike_po
     SHRIKE_REQUIRE(d_x_codes && d_x_scales && d_route_partials && d_workspace, "mx grouped FFN: NULL buffer");
     SHRIKE_REQUIRE(mx_aligned(d_x_codes) && mx_aligned(d_route_partials), "mx grouped FFN: codes and partials must be 16-byte aligned");
     SHRIKE_REQUIRE(reinterpret_cast<uintptr_t>(d_workspace) % 256u == 0, "mx grouped FFN: workspace must be 256-byte aligned");
-    SHRIKE_REQUIRE(uint64_t(query_count) * d <= 0xffffffffull, "mx grouped FFN: %u rows of %u are more than 4 GiB of codes", query_count, d);
+    // (the rows' codes are reached by 32 bits, and past a row's end ahead of the clamp)
+    SHRIKE_REQUIRE(uint64_t(query_count) * d <= 0xffffffffull - 1024u, "mx grouped FFN: %u rows of %u are more than 4 GiB of codes", query_count, d);
     if (query_count == 0 || max_row_tiles == 0) return 0;
     // (an expert's last tile may be partly filled: more tiles than this there cannot be)
     const uint32_t tiles = readable_records(max_row_tiles, uint64_t(query_count) * top_k, moe->desc.num_experts);
