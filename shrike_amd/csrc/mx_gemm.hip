@@ -817,13 +817,13 @@ struct MxRuns {
     MxRun run[1];
 };
 static constexpr size_t mx_runs_bytes(size_t records) { return (sizeof(MxRuns) + records * sizeof(MxRun) + 255u) & ~size_t(255); }
-constexpr uint32_t kRunThreads = 1024, kRunClasses = 16;  // by 16 rows
+constexpr uint32_t kRunThreads = 256, kRunClasses = 16;  // by 16 rows
 
 __global__ __launch_bounds__(kRunThreads) void k_mx_expert_runs(const shrike_row_tile *tiles, const uint32_t *tile_count, uint32_t records, MxRuns *runs) {
     __shared__ uint32_t starts[kRunThreads / 64u], counts[kRunClasses], at[kRunClasses];
     const uint32_t count = min(*tile_count, records), lane = threadIdx.x & 63u, wave = threadIdx.x / 64u;
     if (threadIdx.x < kRunClasses) counts[threadIdx.x] = 0;
-    // rows of the run that starts with record i, or 0; every thread calls it, 1,024 neighbouring records at a time
+    // rows of the run that starts with record i, or 0; every thread calls it, 256 neighbouring records at a time
     auto rows_of = [&](uint32_t i, uint32_t &carried) -> uint32_t {
         const bool there = i < count, start = there && (i == 0 || !goes_on(tiles[i - 1u], tiles[i]));
         const uint64_t in_wave = __ballot(start);
