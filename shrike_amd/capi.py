@@ -20,7 +20,7 @@ META_BF16, META_F16 = 0, 1
 ACT_GELU_TANH, ACT_SILU, ACT_CLAMPED_SWIGLU = 0, 1, 2
 ELEM_BF16, ELEM_F16, ELEM_F32 = 0, 1, 2
 MX_E4M3, MX_E2M1 = 0, 1
-MX_BLOCK, MX_MAX_K = 32, 65536
+MX_BLOCK, MX_MAX_K, MX_MAX_DECODE_TOKENS = 32, 65536, 64
 EMPTY, LOADING, RESIDENT = 0, 1, 2
 
 

@@ -164,3 +164,21 @@ def test_the_reference_on_known_codes():
         assert np.array_equal(R.quantize(R.values(codes, s, fmt), fmt)[0], codes) or fmt == R.E2M1
         top = np.repeat(np.abs(x.reshape(20, -1, 32)).max(-1), 32, axis=1)
         assert np.all(np.abs(R.values(codes, s, fmt) - x) <= most * top)
+
+
+@pytest.mark.parametrize("tokens,refusal", [(capi.MX_MAX_DECODE_TOKENS, None), (capi.MX_MAX_DECODE_TOKENS + 1, "many")])
+def test_decode_takes_so_many_tokens(tokens, refusal):
+    """(As many as it takes are refused for what comes next, the workspace.)"""
+    lib = capi.load()
+    moe, (off, stride, bases) = handle(), experts()
+    refused(lib.shrike_hip_mx_decode_ffn(C.addressof(moe), None, C.byref(bases), stride, A, C.byref(off), A, A, A, None, A, None, A, 0, 128, 64, 4, tokens),
+            refusal or "needed")
+
+
+def test_grouped_refuses_rows_past_4_gib():
+    lib = capi.load()
+    moe, (off, stride, bases) = handle(), experts()
+    routes = capi.HipGroupedRoutes(A, A, A, A, A)
+    for rows in (1 << 25, (1 << 32) // 128 - 8):
+        refused(lib.shrike_hip_mx_grouped_ffn(C.addressof(moe), None, C.byref(bases), stride, C.byref(off), C.byref(routes), 8, A, A, A, A, 1 << 20, rows, 128, 64, 4),
+                "GiB")
