@@ -538,6 +538,48 @@ struct PrefillRoutedExpertWave {
     std::vector<shrike_routed_expert_block> blocks;
     int paddedRows = 0, tailRows = 0;
 };
+// Blocks of 32 elements with a power-of-two scale (E4M3 or E2M1), and what is made of them; the reference has no such format.
+struct MicroscaledBlocks {
+    static void quantize(Stream s, const void *src, uint32_t srcType, uint64_t srcStrideElements, uint32_t format, void *codes, void *scales,
+                         uint32_t rows, uint32_t d) {
+        check(shrike_hip_mx_quantize(s, src, srcType, srcStrideElements, format, codes, scales, rows, d));
+    }
+    static void dequantize(Stream s, const void *codes, const void *scales, uint32_t format, void *out, uint32_t outType,
+                           uint64_t outStrideElements, uint32_t rows, uint32_t d) {
+        check(shrike_hip_mx_dequantize(s, codes, scales, format, out, outType, outStrideElements, rows, d));
+    }
+    // out = x . w^T (+ bias): w E2M1 blocks
+    static void product(Stream s, const void *xCodes, const void *xScales, uint32_t xFormat, const void *wCodes, const void *wScales,
+                        const void *bias, void *out, uint32_t outType, uint64_t outStrideElements, uint32_t rows, uint32_t n, uint32_t k) {
+        check(shrike_hip_mx_product(s, xCodes, xScales, xFormat, wCodes, wScales, bias, out, outType, outStrideElements, rows, n, k));
+    }
+    // residual add and RMS norm, the normalised rows as fp16 (may be null) and as E4M3 blocks
+    static void residualAddRMSNorm(Stream s, const void *hidden, const void *delta, const void *weight, void *sum, void *out, void *codes,
+                                   void *scales, uint32_t d, float eps, uint32_t rows) {
+        check(shrike_hip_residual_add_rmsnorm_bf16w_mx8(s, hidden, delta, weight, sum, out, codes, scales, d, eps, rows));
+    }
+    // an expert's blob of E2M1 projections; returns its size
+    static uint64_t expertOffsets(uint32_t d, uint32_t f, bool additiveBiases, shrike_expert_offsets &offsets) {
+        const uint64_t size = shrike_mx_expert_offsets_make(d, f, additiveBiases, &offsets);
+        check(size ? 0 : EINVAL);
+        return size;
+    }
+    static size_t groupedWorkspaceBytes(uint32_t maxRowTiles, uint32_t f) { return shrike_hip_mx_ffn_workspace_bytes(maxRowTiles, f); }
+    static void encodeGroupedExpertGEMMs(MoE &moe, Stream s, const ExpertPool &pool, const shrike_expert_offsets &offsets,
+                                         const shrike_hip_grouped_routes &routes, uint32_t maxRowTiles, const void *xCodes, const void *xScales,
+                                         void *routePartials, void *workspace, size_t workspaceSize, uint32_t queryCount, uint32_t d, uint32_t f,
+                                         uint32_t topK) {
+        check(shrike_hip_mx_grouped_ffn(moe.handle(), s, pool.bases(), pool.stride(), &offsets, &routes, maxRowTiles, xCodes, xScales,
+                                        routePartials, workspace, workspaceSize, queryCount, d, f, topK));
+    }
+    static size_t decodeWorkspaceBytes(uint32_t tokens, uint32_t topK, uint32_t f) { return shrike_hip_mx_decode_workspace_bytes(tokens, topK, f); }
+    static void encodeDecodeFFN(MoE &moe, Stream s, const ExpertPool &pool, const uint32_t *slots, const shrike_expert_offsets &offsets,
+                                const void *xCodes, const void *xScales, const void *weights, const void *residual, void *y, void *hidden,
+                                void *workspace, size_t workspaceSize, uint32_t d, uint32_t f, uint32_t topK, uint32_t tokens) {
+        check(shrike_hip_mx_decode_ffn(moe.handle(), s, pool.bases(), pool.stride(), slots, &offsets, xCodes, xScales, weights, residual, y,
+                                       hidden, workspace, workspaceSize, d, f, topK, tokens));
+    }
+};
 struct PrefillGroupedRoutedMoE {
     static constexpr int groupedRowTile = 64, groupedTailRowTile = 32;
     static std::vector<PrefillRoutedExpertWave> planExpertWaves(const std::vector<shrike_expert_pair_range> &ranges,

@@ -589,7 +589,9 @@ uint64_t shrike_mx_expert_offsets_make(uint32_t d, uint32_t f, int additive_bias
  * blocks from fp32. x: codes[query_count][d] and scales, as shrike_hip_residual_add_rmsnorm_bf16w_mx8 leaves them. The handle
  * gives the shape, the activation and whether the experts have (bf16) biases; its weight bits play no part. Routes, pool, absent
  * experts and max_row_tiles as there; the workspace holds the activations: 256-byte aligned, at least
- * shrike_hip_mx_ffn_workspace_bytes(max_row_tiles, f). A pair's row depends on its token and its expert alone. */
+ * shrike_hip_mx_ffn_workspace_bytes(max_row_tiles, f). A pair's row depends on its token and its expert alone. The sums that the
+ * activations are made of are the product's: good to some 5e-6, so an activation that close to the middle of two E4M3 values may take
+ * either. */
 size_t shrike_hip_mx_ffn_workspace_bytes(uint32_t max_row_tiles, uint32_t f);
 int shrike_hip_mx_grouped_ffn(shrike_hip_moe *moe, void *stream, const shrike_pool_bases *pool, uint64_t pool_slot_stride,
                               const shrike_expert_offsets *offsets, const shrike_hip_grouped_routes *routes, uint32_t max_row_tiles,
