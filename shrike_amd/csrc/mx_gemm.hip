@@ -314,18 +314,17 @@ __device__ __forceinline__ uint32_t same_cell_pairs(const uint32_t *slots, uint3
     return before % 16u == 0 ? count : 0u;
 }
 
-// Waves take 16 MT rows of x against 16 NT weight rows (gate and up: NT / 2 tiles of each), PARTS of them a part of k each, whose sums meet
-// in LDS: a row's 1,440 bytes are few for one wave, and a call of few rows is a launch and a few latencies (2,880 x 2,880 by one row 4.6 us,
+// Waves take 16 MT rows of x against 16 NT weight rows (gate and up: NT / 2 tiles of each), a part of k each, and their sums meet in LDS: a row's 1,440 bytes are few for one wave, and a call of few rows is a launch and a few latencies (2,880 x 2,880 by one row 4.6 us,
 // by 64 rows 7.9). Gate and up: the rows are those of up to 16 pairs of one expert, whose weights are then read once. Down: one token's, a
 // position behind the other, a row that every column of the instruction holds.
-template <int XF, int MT, int NT, int WAVES, int PARTS, int AHEAD, MxWork WORK, int LEAST = MT == 1 ? 4 : 2>
+template <int XF, int MT, int NT, int WAVES, int AHEAD, MxWork WORK, int LEAST = MT == 1 ? 4 : 2>
 __global__ __launch_bounds__(64 * WAVES, LEAST) void k_mx_few(MxArgs a) {
     constexpr uint32_t kScales = 16u * (NT + MT) * 32u;  // of a wave
     __shared__ __attribute__((aligned(16))) uint8_t s_scales[WAVES * kScales];
-    __shared__ f32x4 s_part[PARTS > 1 ? WAVES : 1][MT * NT][64];
-    const uint32_t wave = wave_index(), group = wave / PARTS, part = wave % PARTS, lane = threadIdx.x & 63u, m = lane & 15u, q = lane >> 4;
+    __shared__ f32x4 s_part[WAVES][MT * NT][64];
+    const uint32_t wave = wave_index(), lane = threadIdx.x & 63u, m = lane & 15u, q = lane >> 4;
     const uint32_t blocks = a.k / kMxBlock, steps = (blocks + 3u) / 4u, row_codes = blocks * 16u;
-    const uint32_t n0 = (blockIdx.x * (WAVES / PARTS) + group) * (WORK == MxWork::kGateUp ? 8u : 16u) * NT;
+    const uint32_t n0 = blockIdx.x * (WORK == MxWork::kGateUp ? 8u : 16u) * NT;
     uint8_t *const lds = s_scales + wave * kScales;
     f32x4 acc[MT][NT];
 #pragma unroll
@@ -350,7 +349,7 @@ __global__ __launch_bounds__(64 * WAVES, LEAST) void k_mx_few(MxArgs a) {
         x_scale_at = x_row(lane % (16u * MT)) * blocks;
         few_steps<XF, MT, NT, AHEAD>(acc, lds, {a.w + size_t(first) * row_codes, a.w_scales + size_t(first) * blocks}, w_at, w_scale_at,
                                      {a.x + size_t(row0) * mx_code_bytes<XF>(a.k), a.x_scales + size_t(row0) * blocks}, x_at, x_scale_at,
-                                     steps * part / PARTS, steps * (part + 1u) / PARTS, blocks);
+                                     steps * wave / WAVES, steps * (wave + 1u) / WAVES, blocks);
     } else if constexpr (WORK == MxWork::kGateUp) {
         const uint32_t cell = a.slots[blockIdx.y];
         if (cell == kSentinel) return;
@@ -362,11 +361,11 @@ __global__ __launch_bounds__(64 * WAVES, LEAST) void k_mx_few(MxArgs a) {
         w_scale_at = (lane >= 8u * NT ? a.off.up_s_off : a.off.gate_s_off) + weight_row(lane % (8u * NT)) * blocks;
         x_at[0] = pair / a.top_k * a.k;
         x_scale_at = pair / a.top_k * blocks;
-        few_steps<XF, MT, NT, AHEAD>(acc, lds, {base, base}, w_at, w_scale_at, {a.x, a.x_scales}, x_at, x_scale_at, steps * part / PARTS, steps * (part + 1u) / PARTS, blocks);
+        few_steps<XF, MT, NT, AHEAD>(acc, lds, {base, base}, w_at, w_scale_at, {a.x, a.x_scales}, x_at, x_scale_at, steps * wave / WAVES, steps * (wave + 1u) / WAVES, blocks);
     } else {
         // the positions' steps one behind the other, an equal part of them a wave; a position's sum is weighted when its steps end
-        const uint32_t all = steps * a.top_k, to = all * (part + 1u) / PARTS;
-        uint32_t at = all * part / PARTS;
+        const uint32_t all = steps * a.top_k, to = all * (wave + 1u) / WAVES;
+        uint32_t at = all * wave / WAVES;
 #pragma unroll
         for (int i = 0; i < NT; ++i) w_at[i] = a.off.down_w_off + weight_row(16u * i + m) * row_codes;
         w_scale_at = a.off.down_s_off + weight_row(lane % (16u * NT)) * blocks;
@@ -390,27 +389,25 @@ __global__ __launch_bounds__(64 * WAVES, LEAST) void k_mx_few(MxArgs a) {
             for (int i = 0; i < NT; ++i) acc[0][i] += weight * sum[0][i];
         }
     }
-    if constexpr (PARTS > 1) {
 #pragma unroll
-        for (int i = 0; i < MT * NT; ++i) s_part[wave][i][lane] = acc[i / NT][i % NT];
-        __syncthreads();
-    }
+    for (int i = 0; i < MT * NT; ++i) s_part[wave][i][lane] = acc[i / NT][i % NT];
+    __syncthreads();
     // the sum of tile i of the wave's rows over the parts of k
     auto total = [&](uint32_t i) {
-        f32x4 v = s_part[group * PARTS][i][lane];
+        f32x4 v = s_part[0][i][lane];
 #pragma unroll
-        for (int p = 1; p < PARTS; ++p) v += s_part[group * PARTS + p][i][lane];
+        for (int p = 1; p < WAVES; ++p) v += s_part[p][i][lane];
         return v;
     };
 
     if constexpr (WORK == MxWork::kGateUp) {
         static_assert(NT == 4 && MT == 1, "a wave's gate and up rows are one MX block of activations");
-        if (part != 0 || n0 >= a.n) return;
+        if (wave != 0) return;
         f32x4 gate[2], up[2];
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
-            gate[i] = PARTS > 1 ? total(i) : acc[0][i];
-            up[i] = PARTS > 1 ? total(2u + i) : acc[0][2u + i];
+            gate[i] = total(i);
+            up[i] = total(2u + i);
             if (a.ebias) {
                 gate[i] += mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.gate_ab_off), n0 + 16u * i + 4u * q);
                 up[i] += mx_bias4(reinterpret_cast<const uint16_t *>(base + a.off.up_ab_off), n0 + 16u * i + 4u * q);
@@ -424,17 +421,16 @@ __global__ __launch_bounds__(64 * WAVES, LEAST) void k_mx_few(MxArgs a) {
             if (q == 0) a.act_scales[size_t(pair) * (a.n / kMxBlock) + n0 / kMxBlock] = uint8_t(b.scale);
         }
     } else if constexpr (WORK == MxWork::kDense) {
-        static_assert(PARTS > 1);
-        for (uint32_t i = part; i < uint32_t(MT * NT); i += PARTS) {
+        for (uint32_t i = wave; i < uint32_t(MT * NT); i += WAVES) {
             const uint32_t row = (blockIdx.y * MT + i / NT) * 16u + m, n = n0 + 16u * (i % NT) + 4u * q;
             const f32x4 v = total(i) + mx_bias4(a.bias, n, a.n);
             if (row < a.rows) mx_store4(a.out + row * a.out_stride, n, a.n, v, a.out_dtype, a.out_whole);
         }
     } else {
-        static_assert(PARTS >= NT && PARTS > 1);
-        if (part >= uint32_t(NT)) return;
-        const uint32_t n = n0 + 16u * part + 4u * q;
-        f32x4 v = total(part);
+        static_assert(WAVES >= NT);
+        if (wave >= uint32_t(NT)) return;
+        const uint32_t n = n0 + 16u * wave + 4u * q;
+        f32x4 v = total(wave);
         if (m != 0 || n >= a.n) return;  // (n and a.n are multiples of four)
         if (a.ebias)
             for (uint32_t p = 0; p < a.top_k; ++p) {
@@ -1143,9 +1139,9 @@ template <int XF>
 static int launch_product(const MxArgs &a, hipStream_t s) {
     const uint64_t columns = (a.n + 255u) / 256u, few = uint64_t((a.n + 15u) / 16u) * ((a.rows + 63u) / 64u);
     if (a.rows <= 16u)
-        hipLaunchKernelGGL((k_mx_few<XF, 1, 1, 8, 8, 4, MxWork::kDense>), dim3((a.n + 15u) / 16u, 1), dim3(512), 0, s, a);
+        hipLaunchKernelGGL((k_mx_few<XF, 1, 1, 8, 4, MxWork::kDense>), dim3((a.n + 15u) / 16u, 1), dim3(512), 0, s, a);
     else if (a.rows <= 64u || few <= (XF == SHRIKE_MX_E4M3 ? 384u : 768u))
-        hipLaunchKernelGGL((k_mx_few<XF, 4, 1, 8, 8, 2, MxWork::kDense>), dim3((a.n + 15u) / 16u, (a.rows + 63u) / 64u), dim3(512), 0, s, a);
+        hipLaunchKernelGGL((k_mx_few<XF, 4, 1, 8, 2, MxWork::kDense>), dim3((a.n + 15u) / 16u, (a.rows + 63u) / 64u), dim3(512), 0, s, a);
     else if (columns * ((a.rows + 63u) / 64u) <= 256u)
         launch_tiles<XF, 2>(a, s);
     else if (columns * ((a.rows + 127u) / 128u) <= 256u)
@@ -1343,15 +1339,15 @@ int shrike_hip_mx_decode_ffn(shrike_hip_moe *moe, void *stream, const shrike_poo
     // 2,048 (128 pairs) 50 and 60. (2 of gpt-oss's tokens, 360, are the other way about: 25.8 and 23.4.)
     const uint32_t pairs = tokens * top_k, workgroups = (f + 63u) / 64u * pairs;
     if (workgroups >= 256u) hipLaunchKernelGGL(k_mx_decode_thin, dim3((f + 63u) / 64u, pairs), dim3(128), MxThinLds::kBytes, s, a);
-    else hipLaunchKernelGGL((k_mx_few<SHRIKE_MX_E4M3, 1, 4, 4, 4, 3, MxWork::kGateUp, 3>), dim3(f / 32u, pairs), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_mx_few<SHRIKE_MX_E4M3, 1, 4, 4, 3, MxWork::kGateUp, 3>), dim3(f / 32u, pairs), dim3(256), 0, s, a);
     SHRIKE_HIP(hipGetLastError());
     a.x = a.act;
     a.x_scales = a.act_scales;
     a.n = d; a.k = f;
     // Down, a token's 32 outputs by eight waves, or 16 by sixteen where those were no more than one a compute unit: 144 workgroups (d 2,304) 8.0 us and
     // 10.5 with half as many, 180 (d 2,880) 10.9 and 13.5, 256 (2 tokens of 2,048) 6.5 and 7.2, 288 13.6 and 10.4, 2,304 (16 tokens) 58 and 38.
-    if (d / 16u * tokens <= 256u) hipLaunchKernelGGL((k_mx_few<SHRIKE_MX_E4M3, 1, 1, 16, 16, 3, MxWork::kDown, 4>), dim3(d / 16u, tokens), dim3(1024), 0, s, a);
-    else hipLaunchKernelGGL((k_mx_few<SHRIKE_MX_E4M3, 1, 2, 8, 8, 3, MxWork::kDown, 4>), dim3((d + 31u) / 32u, tokens), dim3(512), 0, s, a);
+    if (d / 16u * tokens <= 256u) hipLaunchKernelGGL((k_mx_few<SHRIKE_MX_E4M3, 1, 1, 16, 3, MxWork::kDown>), dim3(d / 16u, tokens), dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((k_mx_few<SHRIKE_MX_E4M3, 1, 2, 8, 3, MxWork::kDown>), dim3((d + 31u) / 32u, tokens), dim3(512), 0, s, a);
     SHRIKE_HIP(hipGetLastError());
     return 0;
 }
