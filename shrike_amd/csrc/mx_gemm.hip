@@ -462,9 +462,9 @@ __global__ __launch_bounds__(64 * WAVES, LEAST) void k_mx_few(MxArgs a) {
 // every operand is read from LDS by two waves. A line is a unit of k, 256 of E2M1 codes, 128 of E4M3; two units of either operand have a
 // place, and the next one is asked for while the last one is multiplied. The pieces of a line are swapped about so that 16 rows' same
 // piece lies in 64 different banks.
-// Measured: 4,096 x 4,096 x 2,880 of E4M3 rows 43 us (2,230 TFLOP/s), of which 17 are start, outputs and end; a step of 128 k 1.2 to 1.4 us
-// where its products take 0.9, of E2M1 rows 0.85 and 0.5. Reading the next step's weights ahead of its barrier, or touching lines two steps
-// ahead of their loads, makes no step shorter (the latter a tenth longer): what is left is loads, LDS and products at once.
+// Measured: 4,096 x 4,096 x 2,880 of E4M3 rows 42.5 us (2,270 TFLOP/s), of which 17 are start, outputs and end; a step of 128 k 1.2 to 1.4 us
+// where its products take 0.9, of E2M1 rows 0.85 and 0.5. Reading the next step's weights ahead of its barrier, or rows two tiles ahead, makes
+// no step shorter; touching lines two steps ahead of their loads makes it a tenth longer.
 template <int MT>
 struct MxTileLds {
     static constexpr uint32_t kRows = 32u * MT, kWeights = 256u;
@@ -542,10 +542,35 @@ struct MxTile {
                     sx[b / 4u] |= uint32_t(xs[xs_at + b]) << 8u * (b % 4u);
                 }
         };
+        // Into LDS so that a lane finds the four steps' bytes of its block in one word (read byte by byte, a step each: 43.0 us in place of 42.5 for 4,096 x
+        // 4,096 x 2,880): word j takes bytes j, 4 + j, 8 + j, 12 + j. The last 16 of a row are moved up to where they belong, the last one behind them (the codes
+        // there are zeros).
+        auto by_steps = [&](u32x4 v, uint32_t g) {
+            if (blocks >= 16u && 16u * g > blocks - 16u) {
+                const uint32_t ahead = 16u * g - (blocks - 16u), last = (v[3] >> 24) * 0x01010101u;
+                for (uint32_t i = 0; i < ahead / 4u; ++i) v = u32x4{v[1], v[2], v[3], last};
+                const uint32_t by = ahead % 4u;
+                v = u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], by), __builtin_amdgcn_alignbyte(v[2], v[1], by), __builtin_amdgcn_alignbyte(v[3], v[2], by),
+                          __builtin_amdgcn_alignbyte(last, v[3], by)};
+            }
+            const uint32_t low01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u), high01 = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);
+            const uint32_t low23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u), high23 = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
+            return u32x4{__builtin_amdgcn_perm(low23, low01, 0x05040100u), __builtin_amdgcn_perm(low23, low01, 0x07060302u),
+                         __builtin_amdgcn_perm(high23, high01, 0x05040100u), __builtin_amdgcn_perm(high23, high01, 0x07060302u)};
+        };
         auto store_scales = [&](uint32_t g) {
             uint8_t *to = lds + L::kScales + (g & 1u) * L::kScalePlace;
-            reinterpret_cast<u32x4 *>(to)[threadIdx.x] = sw;
-            if (threadIdx.x < L::kRows) reinterpret_cast<u32x4 *>(to + L::kWeights * 16u)[threadIdx.x] = sx;
+            reinterpret_cast<u32x4 *>(to)[threadIdx.x] = by_steps(sw, g);
+            if (threadIdx.x < L::kRows) reinterpret_cast<u32x4 *>(to + L::kWeights * 16u)[threadIdx.x] = by_steps(sx, g);
+        };
+        // the wave's scales of four steps; the lowest byte is the next one's
+        uint32_t w_scale[8], x_scale[MT];
+        auto fetch_scales = [&](uint32_t g) {
+            const uint8_t *from = lds + L::kScales + (g & 1u) * L::kScalePlace + m * 16u + q * 4u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w_scale[i] = *reinterpret_cast<const uint32_t *>(from + (wn * 8u + i) * 256u);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) x_scale[t] = *reinterpret_cast<const uint32_t *>(from + L::kWeights * 16u + (wm * MT + t) * 256u);
         };
         // A step: 16 rows of x against the wave's 128 weight rows at a time, and between them, one by one, the next units' loads. (All at once they
         // would hold up every wave for as long as the address unit takes.) LAST: the rows may end inside the step; the weights' codes past their end
@@ -555,31 +580,19 @@ struct MxTile {
             const uint32_t half_w = 4u * (s & 1u), half_x = XF == SHRIKE_MX_E4M3 ? 0u : half_w;  // pieces from the unit's start
             const uint8_t *weights = lds + L::kAtW + (s / 2u & 1u) * L::kW + wn * 16384u + m * 128u;
             const uint8_t *rows = lds + (s / kSteps & 1u) * L::kX + wm * (MT * 2048u) + m * 128u;
-            // the lane's block among its row's scales here: past the row's end, the row's last one (its codes are zeros)
-            const uint32_t g = s / 4u, byte = (LAST ? min(4u * s + q, blocks - 1u) : 4u * s + q) - (blocks >= 16u ? min(16u * g, blocks - 16u) : 0u);
-            const uint8_t *scale_w = lds + L::kScales + (g & 1u) * L::kScalePlace + (wn * 128u + m) * 16u + byte;
-            const uint8_t *scale_x = lds + L::kScales + (g & 1u) * L::kScalePlace + (L::kWeights + wm * MT * 16u + m) * 16u + byte;
-            struct Rows {
-                MxFragment<XF> f;
-                uint32_t scale;
-            };
-            auto fetch = [&](Rows &r, int t, int part) {
-                if (part == 0) r.f.piece[0] = *reinterpret_cast<const u32x4 *>(rows + t * 2048u + 16u * ((half_x + q) ^ (m >> 1)));
+            auto fetch = [&](MxFragment<XF> &f, int t, int part) {
+                if (part == 0) f.piece[0] = *reinterpret_cast<const u32x4 *>(rows + t * 2048u + 16u * ((half_x + q) ^ (m >> 1)));
                 if constexpr (XF == SHRIKE_MX_E4M3)
-                    if (part == 1) r.f.piece[1] = *reinterpret_cast<const u32x4 *>(rows + t * 2048u + 16u * ((4u + q) ^ (m >> 1)));
-                if (part == 2) r.scale = scale_x[t * 256u];
+                    if (part == 1) f.piece[1] = *reinterpret_cast<const u32x4 *>(rows + t * 2048u + 16u * ((4u + q) ^ (m >> 1)));
             };
-            Rows now, next;
+            MxFragment<XF> now, next;
 #pragma unroll
-            for (int part = 0; part < 3; ++part) fetch(now, 0, part);
-            next.f = now.f;
-            next.scale = now.scale;
+            for (int part = 0; part < 2; ++part) fetch(now, 0, part);
+            next = now;
             u32x4 wf[8];
-            uint32_t ws[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 wf[i] = *reinterpret_cast<const u32x4 *>(weights + i * 2048u + 16u * ((half_w + q) ^ (m >> 1)));
-                ws[i] = scale_w[i * 256u];
                 if (LAST)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) wf[i][e] = 4u * s + q < blocks ? wf[i][e] : 0u;
@@ -589,18 +602,20 @@ struct MxTile {
                 // between the products, one thing each: the next rows' operands, then loads
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    acc[t][i] = mx_multiply<XF>(wf[i], now.f, acc[t][i], ws[i], now.scale);
+                    acc[t][i] = mx_multiply<XF>(wf[i], now, acc[t][i], w_scale[i], x_scale[t]);
                     __builtin_amdgcn_sched_barrier(0);
-                    if (t + 1 < MT && i < 3) fetch(next, t + 1, i);
+                    if (t + 1 < MT && i < 2) fetch(next, t + 1, i);
                     if (i >= 3) issue<NEXT_X, NEXT_W>(s, 5 * t + i - 3, load_x, load_w);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 // (the products stay ahead of what follows: they have no effect that would keep the compiler from moving them)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) asm volatile("" : "+a"(acc[t][i]));
-                now.f = next.f;  // (one by one: with the structure's padding it would go through memory)
-                now.scale = next.scale;
+                x_scale[t] >>= 8;
+                now = next;
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w_scale[i] >>= 8;
         };
 #pragma unroll
         for (int i = 0; i < MT * 8; ++i) {
@@ -623,7 +638,10 @@ struct MxTile {
             __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0) in the compiler's own count
             if (s % 4u == 0) store_scales(s / 4u);
             wait_loads_and_sync<0>();
-            if (s % 4u == 0 && s + 4u < steps) load_scales(s / 4u + 1u);
+            if (s % 4u == 0) {
+                fetch_scales(s / 4u);
+                if (s + 4u < steps) load_scales(s / 4u + 1u);
+            }
             __builtin_amdgcn_sched_barrier(0);
         };
         auto middle = [&] {
@@ -755,35 +773,36 @@ __device__ __forceinline__ void mx_tile(const MxArgs &a, uint8_t *lds, uint32_t 
                 const shrike_token_expert_pair p = a.pairs[pair0 + min(wm * 16u * MT + 64u * i + lane, rows - 1u)];
                 place[i] = p.token * a.top_k + p.rank;
             }
+        const uint32_t n8 = first + wn * 128u + 8u * m;
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (uint32_t t = 0; t < uint32_t(MT); ++t) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (uint32_t i = 0; i < 8; ++i) {
                 const uint2 h = mx_pack4(tile.acc[t][i] + bias[i], WORK == MxWork::kDense ? a.out_dtype : uint32_t(SHRIKE_ELEM_F16));
                 *reinterpret_cast<uint2 *>(room + (16u * t + m) * 256u + 16u * ((2u * i + q / 2u) ^ m) + q % 2u * 8u) = h;
             }
-        const uint32_t n8 = first + wn * 128u + 8u * m;
 #pragma unroll
-        for (uint32_t j = 0; j < 4u * MT; ++j) {
-            const uint32_t r = 4u * j + q, at = wm * 16u * MT + r;
-            const uint4 v = *reinterpret_cast<const uint4 *>(room + r * 256u + 16u * (m ^ (r & 15u)));
-            const uint32_t slot = uint32_t(__shfl(int(place[MT > 4 ? j / 16u : 0u]), int(r % 64u)));
-            if (at >= rows || n8 >= a.n) continue;
-            uint16_t *to;
-            bool whole = true;
-            if constexpr (WORK == MxWork::kDense) {
-                to = a.out + (row0 + at) * a.out_stride;
-                whole = a.out_whole && n8 + 8u <= a.n;
-            } else {
-                to = a.out + size_t(slot) * a.n;
-            }
-            if (whole) {
-                *reinterpret_cast<uint4 *>(to + n8) = v;
-            } else {
-                const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+            for (uint32_t j = 4u * t; j < 4u * t + 4u; ++j) {
+                const uint32_t r = 4u * j + q, at = wm * 16u * MT + r;
+                const uint4 v = *reinterpret_cast<const uint4 *>(room + r * 256u + 16u * (m ^ (r & 15u)));
+                const uint32_t slot = uint32_t(__shfl(int(place[MT > 4 ? j / 16u : 0u]), int(r % 64u)));
+                if (at >= rows || n8 >= a.n) continue;
+                uint16_t *to;
+                bool whole = true;
+                if constexpr (WORK == MxWork::kDense) {
+                    to = a.out + (row0 + at) * a.out_stride;
+                    whole = a.out_whole && n8 + 8u <= a.n;
+                } else {
+                    to = a.out + size_t(slot) * a.n;
+                }
+                if (whole) {
+                    *reinterpret_cast<uint4 *>(to + n8) = v;
+                } else {
+                    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (uint32_t e = 0; e < 8; ++e)
-                    if (n8 + e < a.n) to[n8 + e] = uint16_t(words[e / 2u] >> 16u * (e % 2u));
+                    for (uint32_t e = 0; e < 8; ++e)
+                        if (n8 + e < a.n) to[n8 + e] = uint16_t(words[e / 2u] >> 16u * (e % 2u));
+                }
             }
         }
     }
