@@ -603,8 +603,8 @@ int shrike_hip_mx_grouped_ffn(shrike_hip_moe *moe, void *stream, const shrike_po
  * y[t]). d_resolved_slots: u32[tokens, top_k], the experts' cells, SHRIKE_SLOT_SENTINEL a position that contributes nothing;
  * d_routing_weights: fp16[tokens, top_k]; residual (NULL = 0), y and hidden (may be NULL): fp16[tokens, d]. The workspace holds the
  * activations: 256-byte aligned, at least shrike_hip_mx_decode_workspace_bytes(). Up to SHRIKE_MX_MAX_DECODE_TOKENS tokens: an
- * expert that several of them route to has its gate and up read once for every 16 of its pairs. Activations round as there. (How many tokens a call has may change the
- * order of the sums over k, and so a result's last bit.) */
+ * expert that several of them route to has its gate and up read once for every 16 of its pairs. Activations round as there. (How many
+ * tokens a call has may change the order of the sums over k, and with it how an activation so close to a middle rounds.) */
 size_t shrike_hip_mx_decode_workspace_bytes(uint32_t tokens, uint32_t top_k, uint32_t f);
 int shrike_hip_mx_decode_ffn(shrike_hip_moe *moe, void *stream, const shrike_pool_bases *pool, uint64_t pool_slot_stride,
                              const uint32_t *d_resolved_slots, const shrike_expert_offsets *offsets, const void *d_x_codes,
