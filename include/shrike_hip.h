@@ -566,7 +566,7 @@ int shrike_hip_mx_dequantize(void *stream, const void *d_codes, const void *d_sc
 /* shrike_hip_residual_add_rmsnorm_bf16w with its rows in 8 bits: sum = fp16(hidden + delta), out = fp16(norm(sum) * weight), the bits
  * of that call, and codes, scales = the E4M3 blocks of `out`. d_sum may be d_hidden (in place); d_delta and d_sum are bound together
  * or both NULL (no add). d_out may be NULL (the router reads fp16 rows, the experts the codes). d: a multiple of 32 up to
- * SHRIKE_MAX_HIDDEN; buffers but d_scales 16-byte aligned. */
+ * SHRIKE_MAX_HIDDEN; rows fewer than 2^24; buffers but d_scales 16-byte aligned. */
 int shrike_hip_residual_add_rmsnorm_bf16w_mx8(void *stream, const void *d_hidden, const void *d_delta, const void *d_weight, void *d_sum,
                                               void *d_out, void *d_codes, void *d_scales, uint32_t d, float eps, uint32_t rows);
 

@@ -223,7 +223,7 @@ int shrike_hip_residual_add_rmsnorm_bf16w_mx8(void *stream, const void *d_hidden
     SHRIKE_REQUIRE(((reinterpret_cast<uintptr_t>(d_hidden) | reinterpret_cast<uintptr_t>(d_delta) | reinterpret_cast<uintptr_t>(d_weight)
                      | reinterpret_cast<uintptr_t>(d_sum) | reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(d_codes)) & 15u) == 0,
                    "rmsnorm mx8: buffers must be 16-byte aligned");
-    SHRIKE_REQUIRE(rows <= 65535u * 1024u, "rmsnorm mx8: %u rows is too many", rows);
+    SHRIKE_REQUIRE(rows <= kMaxNormRows, "rmsnorm mx8: %u rows are too many, %u at most", rows, kMaxNormRows);
     if (rows == 0) return 0;
     MxNormArgs a = {static_cast<const uint16_t *>(d_hidden), static_cast<const uint16_t *>(d_delta), static_cast<const uint16_t *>(d_weight),
                     static_cast<uint16_t *>(d_sum), static_cast<uint16_t *>(d_out), static_cast<uint8_t *>(d_codes),

@@ -7,6 +7,9 @@
 
 namespace shrike {
 
+// Rows of a call, a workgroup of 256 threads each: a launch has fewer than 2^32 threads.
+constexpr uint32_t kMaxNormRows = 0xffffffffu / 256u;
+
 // h[i] = half(hidden[i] + delta[i]) (delta may be null), out[i] = half(h[i] * inv * weight[i]) with
 // inv = 1 / sqrt(mean(h^2) + eps). The sum of squares is fp32: thread t takes the 8-element chunks
 // t, t+256, ... in one fma chain, a wave folds with the xor butterfly 32...1, the four wave sums are
