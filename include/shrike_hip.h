@@ -537,7 +537,7 @@ int shrike_hip_residual_add_f16(void *stream, void *d_hidden, const void *d_delt
  * (residual_add_rmsnorm_bf16w and rmsnorm_bf16w, sources/Shrike/Metal/Primitives/rmsnorm.metal:70-130;
  * called at RealForwardRunner.swift:2852-2858): per row, hidden = fp16(hidden + delta) in place
  * (d_delta NULL: no add), then out = fp16(hidden * rsqrt(mean(hidden^2) + eps) * bf16 weight), the
- * mean in fp32. The decode call is one row; `rows` rows of d elements are done a workgroup each.
+ * mean in fp32. The decode call is one row; `rows` rows of d elements (fewer than 2^24) are done a workgroup each.
  * Bitwise equal to shrike_hip_residual_add_f16 followed by the norm alone, as in the reference. */
 int shrike_hip_residual_add_rmsnorm_bf16w(void *stream, void *d_hidden, const void *d_delta,
                                           const void *d_weight, void *d_out, uint32_t d, float eps,

@@ -25,7 +25,7 @@ extern "C" int shrike_hip_residual_add_rmsnorm_bf16w(void *stream, void *d_hidde
     SHRIKE_REQUIRE(((reinterpret_cast<uintptr_t>(d_hidden) | reinterpret_cast<uintptr_t>(d_delta) | reinterpret_cast<uintptr_t>(d_weight)
                      | reinterpret_cast<uintptr_t>(d_out)) & 15u) == 0,
                    "rmsnorm: buffers must be 16-byte aligned");
-    SHRIKE_REQUIRE(rows <= 65535u * 1024u, "rmsnorm: %u rows is too many", rows);
+    SHRIKE_REQUIRE(rows <= kMaxNormRows, "rmsnorm: %u rows are too many, %u at most", rows, kMaxNormRows);
     if (rows == 0) return 0;
     hipLaunchKernelGGL(k_residual_add_rmsnorm, dim3(rows), dim3(256), 0, as_stream(stream), static_cast<uint16_t *>(d_hidden),
                        static_cast<const uint16_t *>(d_delta), static_cast<const uint16_t *>(d_weight), static_cast<uint16_t *>(d_out),
