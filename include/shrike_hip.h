@@ -581,7 +581,8 @@ int shrike_hip_mx_product(void *stream, const void *d_x_codes, const void *d_x_s
 
 /* An expert's blob of E2M1 projections: gate codes, gate scales, up codes, up scales, down codes, down scales, and the bf16 biases
  * of gate, up and down when asked for, one behind the other. The offsets of affine biases (`*_b_off`) are zero. d and f: multiples
- * of 64. Returns the blob's size, 0 on invalid arguments. */
+ * of 64. Returns the blob's size, 0 on invalid arguments. (A caller's own offsets: codes at multiples of 16 that end at least 128 bytes
+ * below 4 GiB, scales anywhere below 4 GiB, biases at even offsets, all of it within the pool's stride.) */
 uint64_t shrike_mx_expert_offsets_make(uint32_t d, uint32_t f, int additive_biases, shrike_expert_offsets *out);
 
 /* shrike_hip_prefill_grouped_ffn over such experts and 8-bit rows: route_partials[(token * top_k + rank) * d ..] =

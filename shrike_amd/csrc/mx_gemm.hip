@@ -1176,9 +1176,11 @@ static bool mx_aligned(const void *p) { return reinterpret_cast<uintptr_t>(p) % 
 // An expert's blob in a cell: what the codes' 16-byte loads and the cell's size allow.
 static int check_mx_offsets(const shrike_expert_offsets *o, uint64_t stride, uint32_t d, uint32_t f, bool biases) {
     const uint64_t codes = uint64_t(d) * f / 2u, scales = uint64_t(d) * f / kMxBlock;
-    stride = std::min<uint64_t>(stride, 0xffffffffull);  // (the kernels' offsets from a cell's start are 32 bits)
+    // The kernels' offsets from a cell's start are 32 bits, and those of codes reach up to a line past a row's end ahead of the clamp to it.
+    stride = std::min<uint64_t>(stride, 0xffffffffull);
+    const uint64_t codes_end = std::min<uint64_t>(stride, 0xffffffffull - 128u);
     SHRIKE_REQUIRE(o->gate_w_off % 16u == 0 && o->up_w_off % 16u == 0 && o->down_w_off % 16u == 0, "mx experts: code offsets must be multiples of 16");
-    SHRIKE_REQUIRE(o->gate_w_off + codes <= stride && o->up_w_off + codes <= stride && o->down_w_off + codes <= stride
+    SHRIKE_REQUIRE(o->gate_w_off + codes <= codes_end && o->up_w_off + codes <= codes_end && o->down_w_off + codes <= codes_end
                        && o->gate_s_off + scales <= stride && o->up_s_off + scales <= stride && o->down_s_off + scales <= stride,
                    "mx experts: a projection of %u x %u does not fit a cell of %llu bytes", d, f, (unsigned long long)stride);
     if (biases) {
