@@ -541,11 +541,11 @@ struct PrefillRoutedExpertWave {
 // Blocks of 32 elements with a power-of-two scale (E4M3 or E2M1), and what is made of them; the reference has no such format.
 struct MicroscaledBlocks {
     static void quantize(Stream s, const void *src, uint32_t srcType, uint64_t srcStrideElements, uint32_t format, void *codes, void *scales,
-                         uint32_t rows, uint32_t d) {
+                         uint64_t rows, uint32_t d) {
         check(shrike_hip_mx_quantize(s, src, srcType, srcStrideElements, format, codes, scales, rows, d));
     }
     static void dequantize(Stream s, const void *codes, const void *scales, uint32_t format, void *out, uint32_t outType,
-                           uint64_t outStrideElements, uint32_t rows, uint32_t d) {
+                           uint64_t outStrideElements, uint64_t rows, uint32_t d) {
         check(shrike_hip_mx_dequantize(s, codes, scales, format, out, outType, outStrideElements, rows, d));
     }
     // out = x . w^T (+ bias): w E2M1 blocks
