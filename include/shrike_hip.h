@@ -588,8 +588,8 @@ uint64_t shrike_mx_expert_offsets_make(uint32_t d, uint32_t f, int additive_bias
 /* shrike_hip_prefill_grouped_ffn over such experts and 8-bit rows: route_partials[(token * top_k + rank) * d ..] =
  * fp16(down . E4M3(glu(gate . x, up . x))) for every pair of a resident expert, where E4M3(.) quantises a row's activations to MX
  * blocks from fp32. x: codes[query_count][d] and scales, as shrike_hip_residual_add_rmsnorm_bf16w_mx8 leaves them. The handle
- * gives the shape, the activation and whether the experts have (bf16) biases; its weight bits play no part. Routes, pool, absent
- * experts and max_row_tiles as there; the workspace holds the activations and a list of the row tiles: 256-byte aligned, at least
+ * gives the shape (f up to SHRIKE_MX_MAX_K), the activation and whether the experts have (bf16) biases; its weight bits play no part.
+ * Routes, pool, absent experts and max_row_tiles as there; the workspace holds the activations and a list of the row tiles: 256-byte aligned, at least
  * shrike_hip_mx_ffn_workspace_bytes(max_row_tiles, f). A pair's row depends on its token and its expert alone. The sums that the
  * activations are made of are the product's: good to some 5e-6, so an activation that close to the middle of two E4M3 values may take
  * either. */

@@ -1195,6 +1195,8 @@ static int check_mx_experts(const shrike_hip_moe *moe, const shrike_pool_bases *
                             uint32_t f, uint32_t top_k) {
     SHRIKE_REQUIRE(moe && pool && offsets, "mx experts: NULL argument");
     SHRIKE_REQUIRE(d == moe->desc.d && f == moe->desc.f, "mx experts: shape %ux%u differs from the handle's %ux%u", d, f, moe->desc.d, moe->desc.f);
+    // (a tile's 256 rows of activations are reached by 32 bits)
+    SHRIKE_REQUIRE(f <= SHRIKE_MX_MAX_K, "mx experts: f=%u is more than %u", f, SHRIKE_MX_MAX_K);
     SHRIKE_REQUIRE(top_k >= 1 && top_k <= SHRIKE_MAX_TOP_K, "mx experts: topK=%u not in 1...%u", top_k, SHRIKE_MAX_TOP_K);
     SHRIKE_REQUIRE(pool->cells_per_chunk > 0 && stride % 16u == 0, "mx experts: bad pool geometry");
     for (const void *base : pool->base) SHRIKE_REQUIRE(mx_aligned(base), "mx experts: the pool's bases must be 16-byte aligned");

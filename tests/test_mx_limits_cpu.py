@@ -46,3 +46,19 @@ def test_no_expert_s_codes_lie_in_the_last_line_below_4_gib(part, kind):
         else:
             rc = lib.shrike_hip_mx_decode_ffn(C.addressof(moe), None, C.byref(bases), 1 << 33, A, C.byref(off), A, A, A, None, A, None, A, 0, d, f, 4, 3)
         refused(rc, word)
+
+
+@pytest.mark.parametrize("kind", ["grouped", "decode"])
+def test_experts_refuse_longer_rows_of_activations_than_a_product_takes(kind):
+    """The down product's k is f: 256 rows of it in one tile are reached by 32 bits. (The longest is refused for what comes next, the workspace.)"""
+    lib = capi.load()
+    d = 64
+    routes = capi.HipGroupedRoutes(A, A, A, A, A)
+    for f, word in ((capi.MX_MAX_K, "needed"), (capi.MX_MAX_K + 64, "f="), (1 << 25, "f=")):
+        moe = base.handle(d, f)
+        off, stride, bases = base.experts(d, f)
+        if kind == "grouped":
+            rc = lib.shrike_hip_mx_grouped_ffn(C.addressof(moe), None, C.byref(bases), stride, C.byref(off), C.byref(routes), 8, A, A, A, A, 0, 3, d, f, 4)
+        else:
+            rc = lib.shrike_hip_mx_decode_ffn(C.addressof(moe), None, C.byref(bases), stride, A, C.byref(off), A, A, A, None, A, None, A, 0, d, f, 4, 3)
+        refused(rc, word)
