@@ -8,6 +8,7 @@ namespace shrike {
 
 constexpr uint32_t kMxBlock = 32;
 
+// 8 bytes from any address (scales lie anywhere)
 typedef uint32_t u32x2_by1 __attribute__((ext_vector_type(2), aligned(1)));
 
 template <int FORMAT>

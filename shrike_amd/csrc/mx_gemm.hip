@@ -633,7 +633,6 @@ struct MxTile {
         const std::true_type yes;
         const std::false_type no;
         const std::integral_constant<bool, kSteps == 1u> one;
-        const std::integral_constant<bool, kSteps == 2u> two;
         auto turn = [&](uint32_t s) {
             __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0) in the compiler's own count
             if (s % 4u == 0) store_scales(s / 4u);
@@ -964,7 +963,6 @@ __device__ __forceinline__ void mx_thin(const MxArgs &a, uint8_t *lds, uint32_t 
     uint2 sw[3], sx[3];
     auto scales_from = [&](uint32_t c) { return blocks >= 8u ? min(8u * c, blocks - 8u) : 0u; };
     auto load_scales = [&](uint32_t c) {
-        typedef uint32_t u32x2_by1 __attribute__((ext_vector_type(2), aligned(1)));
         if (blocks >= 8u) {
 #pragma unroll
             for (uint32_t i = 0; i < 3; ++i) {
