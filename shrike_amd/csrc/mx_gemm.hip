@@ -19,6 +19,7 @@
 #include "mx_common.h"
 #include "prefill_common.h"
 
+#include <cstddef>
 #include <type_traits>
 
 namespace shrike {
@@ -1189,6 +1190,8 @@ static int check_mx_offsets(const shrike_expert_offsets *o, uint64_t stride, uin
     return 0;
 }
 
+// (of a handle, these calls read the description alone, and first of all: a bare one at its head is refused as a handle's would be)
+static_assert(offsetof(shrike_hip_moe, desc) == 0);
 static int check_mx_experts(const shrike_hip_moe *moe, const shrike_pool_bases *pool, uint64_t stride, const shrike_expert_offsets *offsets, uint32_t d,
                             uint32_t f, uint32_t top_k) {
     SHRIKE_REQUIRE(moe && pool && offsets, "mx experts: NULL argument");
