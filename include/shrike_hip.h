@@ -566,7 +566,8 @@ int shrike_hip_mx_dequantize(void *stream, const void *d_codes, const void *d_sc
 /* shrike_hip_residual_add_rmsnorm_bf16w with its rows in 8 bits: sum = fp16(hidden + delta), out = fp16(norm(sum) * weight), the bits
  * of that call, and codes, scales = the E4M3 blocks of `out`. d_sum may be d_hidden (in place); d_delta and d_sum are bound together
  * or both NULL (no add). d_out may be NULL (the router reads fp16 rows, the experts the codes). d: a multiple of 32 up to
- * SHRIKE_MAX_HIDDEN; rows fewer than 2^24; buffers but d_scales 16-byte aligned. */
+ * SHRIKE_MAX_HIDDEN; rows fewer than 2^24; buffers but d_scales 16-byte aligned. As there the sum of squares is fp32: of 4,096 x 2,304
+ * random outputs some 450 are the other fp16 neighbour of what 64 bits throughout give, and up to 5 have another code. */
 int shrike_hip_residual_add_rmsnorm_bf16w_mx8(void *stream, const void *d_hidden, const void *d_delta, const void *d_weight, void *d_sum,
                                               void *d_out, void *d_codes, void *d_scales, uint32_t d, float eps, uint32_t rows);
 
@@ -589,10 +590,12 @@ uint64_t shrike_mx_expert_offsets_make(uint32_t d, uint32_t f, int additive_bias
  * fp16(down . E4M3(glu(gate . x, up . x))) for every pair of a resident expert, where E4M3(.) quantises a row's activations to MX
  * blocks from fp32. x: codes[query_count][d] and scales, as shrike_hip_residual_add_rmsnorm_bf16w_mx8 leaves them. The handle
  * gives the shape (f up to SHRIKE_MX_MAX_K), the activation and whether the experts have (bf16) biases; its weight bits play no part.
- * Routes, pool, absent experts and max_row_tiles as there; the workspace holds the activations and a list of the row tiles: 256-byte aligned, at least
- * shrike_hip_mx_ffn_workspace_bytes(max_row_tiles, f). A pair's row depends on its token and its expert alone. The sums that the
+ * Routes, pool, absent experts and max_row_tiles as there, but for at most 65,535 row tiles of the call's pairs; query_count * d is at
+ * most 2^32 - 1,025 (x is reached by 32 bits). The workspace holds the activations and a list of the row tiles: 256-byte aligned, at
+ * least shrike_hip_mx_ffn_workspace_bytes(max_row_tiles, f). A pair's row depends on its token and its expert alone. The sums that the
  * activations are made of are the product's: good to some 5e-6, so an activation that close to the middle of two E4M3 values may take
- * either. */
+ * either, and of random rows one in some 10,000 does: outputs are then off by 5e-4 to 8e-4 of their norm, where sums good to fp32 leave the
+ * 2e-4 of their rounding to fp16. */
 size_t shrike_hip_mx_ffn_workspace_bytes(uint32_t max_row_tiles, uint32_t f);
 int shrike_hip_mx_grouped_ffn(shrike_hip_moe *moe, void *stream, const shrike_pool_bases *pool, uint64_t pool_slot_stride,
                               const shrike_expert_offsets *offsets, const shrike_hip_grouped_routes *routes, uint32_t max_row_tiles,
@@ -604,8 +607,9 @@ int shrike_hip_mx_grouped_ffn(shrike_hip_moe *moe, void *stream, const shrike_po
  * y[t]). d_resolved_slots: u32[tokens, top_k], the experts' cells, SHRIKE_SLOT_SENTINEL a position that contributes nothing;
  * d_routing_weights: fp16[tokens, top_k]; residual (NULL = 0), y and hidden (may be NULL): fp16[tokens, d]. The workspace holds the
  * activations: 256-byte aligned, at least shrike_hip_mx_decode_workspace_bytes(). Up to SHRIKE_MX_MAX_DECODE_TOKENS tokens: an
- * expert that several of them route to has its gate and up read once for every 16 of its pairs. Activations round as there. (How many
- * tokens a call has may change the order of the sums over k, and with it how an activation so close to a middle rounds.) */
+ * expert that several of them route to has its gate and up read once for every 16 of its pairs, its down once a pair. Activations
+ * round as there. (How many tokens a call has may change the order of the sums over k, and with it how an activation so close to a
+ * middle rounds.) */
 size_t shrike_hip_mx_decode_workspace_bytes(uint32_t tokens, uint32_t top_k, uint32_t f);
 int shrike_hip_mx_decode_ffn(shrike_hip_moe *moe, void *stream, const shrike_pool_bases *pool, uint64_t pool_slot_stride,
                              const uint32_t *d_resolved_slots, const shrike_expert_offsets *offsets, const void *d_x_codes,

@@ -207,7 +207,10 @@ __device__ __forceinline__ uint32_t few_scale_byte(uint32_t b, uint32_t start, u
 // Steps [from, to) of a wave's NT tiles of 16 weight rows against its MT tiles of rows of x, `blocks` blocks long: AHEAD steps on their way.
 // Codes come straight from memory into the operands' registers: 16 neighbouring lanes want a piece each of 16 rows, which takes the
 // address unit a cycle a lane, so that a compute unit takes 16 bytes a cycle: enough for weights that are read once. The scales would
-// cost as many cycles again, a byte each, and come through LDS. All the addresses are those of a lane's row.
+// cost as many cycles again, a byte each, and come through LDS. All the addresses are those of a lane's row. The rows of x take the same
+// road, and more of it: a k of 16 weight rows is 8 bytes, of 16 rows of E4M3 16, of E2M1 8. With one tile of E4M3 rows a third of the
+// bytes are weights', with four a ninth, and that bounds calls of many weights (201,088 x 2,880 by 1, 16, 17 and 64 E4M3 rows 98, 140, 232 and
+// 339 us, 3.1 to 0.9 TB/s of weights). Down's row, which every column of the instruction holds, is asked for sixteen times.
 struct MxFewRows {
     const uint8_t *codes, *scales;  // what the offsets count from
 };
@@ -464,7 +467,7 @@ __global__ __launch_bounds__(64 * WAVES, LEAST) void k_mx_few(MxArgs a) {
 // place, and the next one is asked for while the last one is multiplied. The pieces of a line are swapped about so that 16 rows' same
 // piece lies in 64 different banks.
 // Measured: 4,096 x 4,096 x 2,880 of E4M3 rows 42.5 us (2,270 TFLOP/s), of which 17 are start, outputs and end; a step of 128 k 1.2 to 1.4 us
-// where its products take 0.9, of E2M1 rows 0.85 and 0.5. Reading the next step's weights ahead of its barrier, or rows two tiles ahead, makes
+// where its products take 0.9, of E2M1 rows 0.85 and 0.6. Reading the next step's weights ahead of its barrier, or rows two tiles ahead, makes
 // no step shorter; touching lines two steps ahead of their loads makes it a tenth longer.
 template <int MT>
 struct MxTileLds {
@@ -1152,6 +1155,14 @@ static void launch_tiles(const MxArgs &a, hipStream_t s) {
 // 1,536 (288 workgroups of 64 x 256)      101   | 54.8              36.7 | 33.6 25.1 | 21.0 38.7 | 29.2
 // 2,048                                   134   | 72.3              36.9 | 34.2 26.2 | 22.1 39.0 | 29.9
 // Few workgroups read the rows once each: 384 of them from E4M3's bytes, 768 from E2M1's, are where that costs as much as the tiles' start.
+// Up to 64 rows that kernel is taken however many workgroups it has, and of many outputs it loses by that. The same two, calls back to back over
+// three sets of weights:
+//    17 | 64 rows of  2,880 x 2,880   E4M3  6.6,  7.7 (tiles 14.1, 14.9)   E2M1  5.6,  6.3 (12.4, 13.1)
+//                     8,192 x 2,880        10.4, 13.8       (17.7, 18.5)         7.3, 10.4 (16.7, 17.8)
+//                    32,768 x 2,304        33.1, 51.4       (15.7, 16.5)        19.3, 27.3 (14.3, 15.0)
+//                   201,088 x 2,880         232,  339       ( 148,  158)         134,  243 ( 123,  131)
+//     1 | 16 rows of 32,768 x 2,304        13.7, 18.4       (15.3, 15.7)        12.4, 14.5 (14.1, 14.2)
+//                   201,088 x 2,880          98,  140       ( 147,  149)          94,  119 ( 121,  123)
 // Of the tiles the lowest that are dealt out in one go: a compute unit takes one at a time.
 template <int XF>
 static int launch_product(const MxArgs &a, hipStream_t s) {
@@ -1370,6 +1381,8 @@ int shrike_hip_mx_decode_ffn(shrike_hip_moe *moe, void *stream, const shrike_poo
     a.n = d; a.k = f;
     // Down, a token's 32 outputs by eight waves, or 16 by sixteen where those were no more than one a compute unit: 144 workgroups (d 2,304) 8.0 us and
     // 10.5 with half as many, 180 (d 2,880) 10.9 and 13.5, 256 (2 tokens of 2,048) 6.5 and 7.2, 288 13.6 and 10.4, 2,304 (16 tokens) 58 and 38.
+    // Every pair reads its expert, however many share it: with few experts that is what bounds a batch (gpt-oss's down, 16 tokens 67 us and 64 tokens 205,
+    // where the experts that they use are 25 and 29 us of bytes; 16 tokens over 8 experts of 2,048 x 1,024, all of them each, 27, 2 of bytes).
     if (d / 16u * tokens <= 256u) hipLaunchKernelGGL((k_mx_few<SHRIKE_MX_E4M3, 1, 1, 16, 3, MxWork::kDown>), dim3(d / 16u, tokens), dim3(1024), 0, s, a);
     else hipLaunchKernelGGL((k_mx_few<SHRIKE_MX_E4M3, 1, 2, 8, 3, MxWork::kDown>), dim3((d + 31u) / 32u, tokens), dim3(512), 0, s, a);
     SHRIKE_HIP(hipGetLastError());
