@@ -50,6 +50,12 @@ enum { SHRIKE_MX_E4M3 = 0, SHRIKE_MX_E2M1 = 1 };
 #define SHRIKE_MX_BLOCK 32u
 #define SHRIKE_MX_MAX_K 65536u
 #define SHRIKE_MX_MAX_DECODE_TOKENS 64u
+/* Scores of shrike_hip_route_rows, and its limits. */
+enum { SHRIKE_SCORES_SOFTMAX = 0, SHRIKE_SCORES_SIGMOID = 1 };
+#define SHRIKE_ROUTE_MAX_EXPERTS 1024u
+#define SHRIKE_ROUTE_MAX_TOP_K 32u
+#define SHRIKE_ROUTE_MAX_GROUPS 64u
+#define SHRIKE_AFFINE4_MAX_K 65536u
 enum { SHRIKE_RESIDENCY_EMPTY = 0, SHRIKE_RESIDENCY_LOADING = 1, SHRIKE_RESIDENCY_RESIDENT = 2 };
 
 const char *shrike_hip_last_error(void);
@@ -615,6 +621,47 @@ int shrike_hip_mx_decode_ffn(shrike_hip_moe *moe, void *stream, const shrike_poo
                              const uint32_t *d_resolved_slots, const shrike_expert_offsets *offsets, const void *d_x_codes,
                              const void *d_x_scales, const void *d_routing_weights, const void *d_residual, void *d_y, void *d_hidden,
                              void *d_workspace, size_t workspace_bytes, uint32_t d, uint32_t f, uint32_t top_k, uint32_t tokens);
+
+/* ------------------------------------------- routing from logits, and products with 4-bit weights and group scales
+ * NO COUNTERPART IN THE REFERENCE: its routers make their logits themselves, choose among all experts and always renormalise, and its
+ * dense 4-bit projections are its shared expert's and attention's. These two take any producer's logits and any projection of the format. */
+
+/* How a row of logits becomes routes. With l the logits and b the bias (NULL: none), a NaN standing for -inf and +inf for the largest fp32:
+ *   score s[e] = 1 / (1 + exp(-l[e])), or the softmax of l over the row; 0 where l[e] is -inf
+ *   choice c[e] = s[e] + b[e] in 64 bits with a bias, l[e] without one (both scores rise with l); larger first, equal ones lower index first
+ * An expert whose l or b is -inf is out of service: it stands behind all others and its weight is 0. `groups` groups of num_experts / groups
+ * neighbours each (1: none) are compared by their best choice (group_top 1) or by the sum in 64 bits of their two best s[e] + b[e]
+ * (group_top 2; what is missing of the two counts 0, a group with nobody in service comes last), equal ones lower index first, and only
+ * the kept_groups best take part. Of these the top_k first are the route, in that order. weight = scaling * s, or with `renormalize` scaling * s /
+ * (the sum of the chosen s), 0 where nothing is in service. The bias takes part in the choice only. */
+typedef struct {
+    uint32_t num_experts;  /* 1 ... SHRIKE_ROUTE_MAX_EXPERTS */
+    uint32_t top_k;        /* 1 ... SHRIKE_ROUTE_MAX_TOP_K, at most the kept groups' experts */
+    uint32_t scores;       /* SHRIKE_SCORES_* */
+    uint32_t groups;       /* 1 ... SHRIKE_ROUTE_MAX_GROUPS, a divisor of num_experts */
+    uint32_t kept_groups;  /* 1 ... groups */
+    uint32_t group_top;    /* 1 | 2 */
+    uint32_t renormalize;
+    float scaling;
+} shrike_route_desc;
+/* Routes of `rows` rows of logits (fp32, fp16 or bf16, SHRIKE_ELEM_*), logits_stride_elements apart, any address of their own size; d_bias:
+ * [num_experts] of bias_dtype, or NULL. out_indices: u32[rows, top_k]; out_weights: [rows, top_k] of weights_dtype. They feed
+ * shrike_hip_group_pairs and shrike_hip_moe_resolve_batch as the routers' outputs do (fp16 weights). `desc` is read at the call. A row's routes
+ * depend on that row alone. */
+int shrike_hip_route_rows(void *stream, const shrike_route_desc *desc, const void *d_logits, uint32_t logits_dtype, uint64_t logits_stride_elements,
+                          const void *d_bias, uint32_t bias_dtype, uint32_t *d_out_indices, void *d_out_weights, uint32_t weights_dtype,
+                          uint32_t rows);
+
+/* out[r, i] = sum over k of x[r, k] * w[i, k], + bias[i] (16-bit [n] of meta_dtype, may be NULL), for 4-bit rows with a scale and a bias a group:
+ * w[i, k] = code * scales[i, k / group_size] + biases[i, k / group_size], or (code - 8) * scale where w->biases is NULL (symmetric weights).
+ * w->weights: codes u8[n, k / 2], 16-byte aligned; scales and biases: 16-bit [n, k / group_size] of meta_dtype, all without gaps. group_size: 32,
+ * 64 (this library's own) or 128; k: a multiple of group_size up to SHRIKE_AFFINE4_MAX_K; n up to 2^24; rows up to 2^22. x: fp16 or bf16, rows at 16-byte
+ * aligned addresses, x_stride_elements apart (at most 2^36); out: fp16, bf16 or fp32, rows out_stride_elements apart (what lies between them is left as it
+ * is). The codes are never rounded: products of a group are summed and scaled in fp32 and the result is rounded once. The order of these sums
+ * depends on rows, n and k, so calls of other sizes may differ in last places; the same call gives the same bits. */
+int shrike_hip_affine4_product(void *stream, const void *d_x, uint32_t x_dtype, uint64_t x_stride_elements, const shrike_projection *w,
+                               uint32_t meta_dtype, uint32_t group_size, const void *d_bias, void *d_out, uint32_t out_dtype,
+                               uint64_t out_stride_elements, uint32_t rows, uint32_t n, uint32_t k);
 
 /* ----------------------------------------------------------------- plumbing
  * Device memory, streams, events and graphs for hosts without a HIP binding of

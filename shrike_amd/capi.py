@@ -21,6 +21,9 @@ ACT_GELU_TANH, ACT_SILU, ACT_CLAMPED_SWIGLU = 0, 1, 2
 ELEM_BF16, ELEM_F16, ELEM_F32 = 0, 1, 2
 MX_E4M3, MX_E2M1 = 0, 1
 MX_BLOCK, MX_MAX_K, MX_MAX_DECODE_TOKENS = 32, 65536, 64
+SCORES_SOFTMAX, SCORES_SIGMOID = 0, 1
+ROUTE_MAX_EXPERTS, ROUTE_MAX_TOP_K, ROUTE_MAX_GROUPS = 1024, 32, 64
+AFFINE4_MAX_K = 65536
 EMPTY, LOADING, RESIDENT = 0, 1, 2
 
 
@@ -54,6 +57,11 @@ class MoEDesc(C.Structure):
                 ("activation", C.c_uint32), ("expert_additive_biases", C.c_uint32),
                 ("sigmoid_router_scores", C.c_uint32), ("routed_scaling_factor", C.c_float),
                 ("event_gated_io", C.c_uint32)]
+
+
+class RouteDesc(C.Structure):
+    _fields_ = [("num_experts", C.c_uint32), ("top_k", C.c_uint32), ("scores", C.c_uint32), ("groups", C.c_uint32),
+                ("kept_groups", C.c_uint32), ("group_top", C.c_uint32), ("renormalize", C.c_uint32), ("scaling", C.c_float)]
 
 
 class DecodeLayerArgs(C.Structure):
@@ -345,6 +353,8 @@ SIGNATURES = {
     "shrike_hip_mx_decode_workspace_bytes": (C.c_size_t, [_U32, _U32, _U32]),
     "shrike_hip_mx_decode_ffn": (C.c_int, [_VP, _VP, C.POINTER(PoolBases), _U64, _VP, C.POINTER(ExpertOffsets), _VP, _VP, _VP, _VP, _VP,
                                            _VP, _VP, C.c_size_t, _U32, _U32, _U32, _U32]),
+    "shrike_hip_route_rows": (C.c_int, [_VP, C.POINTER(RouteDesc), _VP, _U32, _U64, _VP, _U32, _VP, _VP, _U32, _U32]),
+    "shrike_hip_affine4_product": (C.c_int, [_VP, _VP, _U32, _U64, C.POINTER(Projection), _U32, _U32, _VP, _VP, _U32, _U64, _U32, _U32, _U32]),
     "shrike_hip_malloc": (_VP, [_U64]),
     "shrike_hip_free": (C.c_int, [_VP]),
     "shrike_hip_host_alloc": (_VP, [_U64]),

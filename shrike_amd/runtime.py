@@ -595,3 +595,19 @@ def mx_product(x_codes, x_scales, x_format: int, w_codes, w_scales, bias, out, o
     check(capi.load().shrike_hip_mx_product(stream.handle if stream else None, ptr(x_codes), ptr(x_scales), x_format, ptr(w_codes),
                                             ptr(w_scales), ptr(bias), ptr(out), out_dtype, out_stride_elements, rows, n, k),
           "shrike_hip_mx_product")
+
+
+def route_rows(desc: capi.RouteDesc, logits, logits_dtype: int, logits_stride_elements: int, bias, bias_dtype: int, out_indices, out_weights,
+               weights_dtype: int, rows: int, stream: Stream | None = None) -> None:
+    """Rows of capi.ELEM_* logits into top_k expert indices (u32) and weights (capi.ELEM_*) each, by `desc`; bias may be None."""
+    check(capi.load().shrike_hip_route_rows(stream.handle if stream else None, C.byref(desc), ptr(logits), logits_dtype, logits_stride_elements,
+                                            ptr(bias), bias_dtype, ptr(out_indices), ptr(out_weights), weights_dtype, rows), "shrike_hip_route_rows")
+
+
+def affine4_product(x, x_dtype: int, x_stride_elements: int, codes, scales, biases, meta_dtype: int, group_size: int, bias, out, out_dtype: int,
+                    out_stride_elements: int, rows: int, n: int, k: int, stream: Stream | None = None) -> None:
+    """out[rows, n] = x . w^T (+ bias), w 4-bit codes with scales and biases (None: symmetric) a group, of meta_dtype as `bias` is."""
+    w = Projection(ptr(codes), ptr(scales), ptr(biases))
+    check(capi.load().shrike_hip_affine4_product(stream.handle if stream else None, ptr(x), x_dtype, x_stride_elements, C.byref(w), meta_dtype,
+                                                 group_size, ptr(bias), ptr(out), out_dtype, out_stride_elements, rows, n, k),
+          "shrike_hip_affine4_product")
