@@ -72,8 +72,8 @@ __device__ __forceinline__ float affine4_add(const uint4 &v, float c) {
             const h2_t one = {_Float16(1.0f), _Float16(1.0f)};
             c = __builtin_amdgcn_fdot2(as_h2(w[i]), one, c, false);
         } else {
-            c = __fadd_rn(c, __uint_as_float(w[i] << 16));
-            c = __fadd_rn(c, __uint_as_float(w[i] & 0xffff0000u));
+            const bf2_t one = {__bf16(1.0f), __bf16(1.0f)};
+            c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2_t, w[i]), one, c, false);
         }
     }
     return c;
@@ -383,9 +383,425 @@ static int launch_few(const Affine4Args &args, hipStream_t s) {
     SHRIKE_HIP(hipGetLastError());
     return 0;
 }
+// ------------------------------------------------------------------ many rows
+//
+// 32 MT WM rows against 32 NT WN outputs a workgroup of WM x WN waves, 32 MT x 32 NT a wave. Rows and codes come through LDS, a step of 64 k of the rows
+// two steps ahead in three places, two steps of the codes (64 bytes a row) in two. A chunk is eight chains (a chain is a group's products, or
+// half a group's of 128): its scales are a lane's own loads, a chunk ahead, and the bias term is added a chunk behind from the sums of the rows' groups,
+// which the waves form from the operands that they hold, WN waves a share of the tile's rows each.
+// The lane's number, new at every call
+__device__ __forceinline__ uint32_t lane_number() {
+    uint32_t l;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+    return l;
+}
+
+template <int MT, int NT, int WM, int WN, int P>
+struct TileLds {
+    static constexpr uint32_t kRows = 32u * MT * WM, kOuts = 32u * NT * WN, kWaves = WM * WN;
+    static constexpr uint32_t kX = kRows * 128u;    // a step's rows
+    static constexpr uint32_t kB = kOuts * 64u;     // two steps' codes
+    static constexpr uint32_t kSums = kRows * 48u;  // a chunk's sums, three bf16 terms each
+    static constexpr uint32_t kUnits = (P + 2u) / 2u;  // places of the codes: what is asked for beside a step is needed after its rows
+    static constexpr uint32_t kCodes = P * kX, kSum = kCodes + kUnits * kB, kScales = kSum + 2u * kSums, kBytes = kScales + 2u * kOuts * 16u;
+    static constexpr int kLoadsX = int(kX / 1024u / kWaves), kLoadsB = int(kB / 1024u / kWaves);  // of a wave, a step (two steps)
+    static_assert(kLoadsX * 1024u * kWaves == kX && kLoadsB * 1024u * kWaves == kB && kBytes <= 160u * 1024u);
+    static_assert(kWaves * 32u * (32u * NT * 4u + 16u) <= kBytes, "the outputs on their way out fit");
+};
+
+template <int XT, int GROUP, int MT, int NT, int WM, int WN, int P>
+__global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(Affine4Args a) {
+    typedef TileLds<MT, NT, WM, WN, P> L;
+    constexpr bool SUB32 = GROUP == 32;
+    constexpr uint32_t kSteps = SUB32 ? 4u : 8u;               // of a chunk
+    constexpr uint32_t kMetas = GROUP == 128 ? 4u : 8u;        // a chunk's scales
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // (of a size that the compiler does not know: else it takes sums to the accumulation registers and back)
+    const uint32_t lane = threadIdx.x & 63u, col = lane & 31u, half = lane >> 5;
+    const uint32_t wave = wave_index(), wm = wave / WN, wn = wave % WN;
+    const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)lds));
+    const uint32_t steps = (a.k + 63u) / 64u, chunks = (steps + kSteps - 1u) / kSteps, groups = a.k / uint32_t(GROUP);
+    const uint32_t row0 = blockIdx.y * L::kRows, n0 = blockIdx.x * L::kOuts, rows = min(a.rows - row0, L::kRows);
+
+    // ---- what the wave asks for: eight rows of x a load (eight lanes a row, pieces xor-ed with half the row's number), sixteen of codes
+    // (four lanes a row, xor-ed with a quarter of it). Rows and outputs past the last are the last again; past k stands a row's last piece.
+    const uint32_t pieces = a.k / 8u, code_pieces = a.k / 32u;
+    const uint8_t *const x = reinterpret_cast<const uint8_t *>(a.x + uint64_t(row0) * a.x_stride);
+    const uint8_t *const codes = a.codes + uint64_t(n0) * (a.k / 2u);
+    // (The offsets are formed again from the lane's number at every use: held in registers, they are spilled.)
+    const uint32_t stride = uint32_t(a.x_stride) * 2u, row_bytes = a.k / 2u;
+    auto load_x = [&](uint32_t place, uint32_t g) {
+        const uint32_t l = lane_number(), first = 8u * wave * L::kLoadsX, piece = (l & 7u) ^ (4u * (wave * L::kLoadsX & 1u) + (l >> 4));
+        const uint32_t to = lds0 + place * L::kX + wave * L::kLoadsX * 1024u;
+        const uint8_t *const from = x + size_t(g) * 128u;
+        if (rows == L::kRows && (!SUB32 || 8u * g + 8u <= pieces)) {
+            const uint32_t row = (first + (l >> 3)) * stride, even = row + piece * 16u, odd = row + (piece ^ 4u) * 16u;
+#pragma unroll
+            for (uint32_t j = 0; j < L::kLoadsX; ++j) lds_load16(to + j * 1024u, from + size_t(8u * j) * stride, j % 2u ? odd : even);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < L::kLoadsX; ++j)
+                lds_load16(to + j * 1024u, from, min(first + 8u * j + (l >> 3), rows - 1u) * stride + min(j % 2u ? piece ^ 4u : piece, pieces - 1u - 8u * g) * 16u);
+        }
+    };
+    auto load_b = [&](uint32_t place, uint32_t two) {
+        const uint32_t l = lane_number(), first = 16u * wave * L::kLoadsB, piece = (l & 3u) ^ (l >> 4);
+        const uint32_t to = lds0 + L::kCodes + place * L::kB + wave * L::kLoadsB * 1024u;
+        const uint8_t *const from = codes + size_t(two) * 64u;
+        if (n0 + L::kOuts <= a.n && 4u * two + 4u <= code_pieces) {
+            const uint32_t at = (first + (l >> 2)) * row_bytes + piece * 16u;
+#pragma unroll
+            for (uint32_t j = 0; j < L::kLoadsB; ++j) lds_load16(to + j * 1024u, from + size_t(16u * j) * row_bytes, at);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < L::kLoadsB; ++j)
+                lds_load16(to + j * 1024u, from, min(first + 16u * j + (l >> 2), a.n - 1u - n0) * row_bytes + min(piece, code_pieces - 1u - 4u * two) * 16u);
+        }
+    };
+
+    // ---- a chunk's scales and biases of the lane's outputs
+    const uint32_t n_first = n0 + wn * 32u * NT;
+    const bool active = n_first < a.n;
+    const uint32_t n_base = min(n_first, a.n - 1u);
+    const buffer_t scales = affine4_buffer(a.scales, uint64_t(n_base) * groups * 2u, uint64_t(a.n) * groups * 2u);
+    const buffer_t biases = a.biases ? affine4_buffer(a.biases, uint64_t(n_base) * groups * 2u, uint64_t(a.n) * groups * 2u) : scales;
+    struct Metas {
+        uint32_t v[NT][kMetas / 2];
+    };
+    auto load_metas = [&](Metas &m, buffer_t from, uint32_t chunk) {
+        const uint32_t g = chunk * kMetas, l = lane_number() & 31u;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const uint32_t at = (min(n_first + 32u * i + l, a.n - 1u) - n_base) * groups * 2u;
+            if (g + kMetas > groups) {
+#pragma unroll
+                for (uint32_t j = 0; j < kMetas; ++j) {
+                    const uint32_t v = __builtin_amdgcn_raw_buffer_load_b16(from, at, min(g + j, groups - 1u) * 2u, 0);
+                    m.v[i][j / 2u] = j % 2u ? m.v[i][j / 2u] | v << 16 : v;
+                }
+            } else if constexpr (kMetas == 8u) {
+                const uint4 v = affine4_load16(from, at, g * 2u);
+                m.v[i][0] = v.x;
+                m.v[i][1] = v.y;
+                m.v[i][2] = v.z;
+                m.v[i][3] = v.w;
+            } else {
+                const auto v = __builtin_amdgcn_raw_buffer_load_b64(from, at, g * 2u, 0);
+                m.v[i][0] = v[0];
+                m.v[i][1] = v[1];
+            }
+        }
+    };
+    // of chain c of the chunk
+    auto meta_at = [&](const Metas &m, int i, uint32_t c) {
+        const uint32_t j = GROUP == 128 ? c / 2u : c;
+        return meta_f32(uint16_t(m.v[i][j / 2u] >> 16u * (j % 2u)), a.meta);
+    };
+    // A chunk's scales wait in LDS, where the lane that wrote them reads them (both halves write the same): in registers something else is spilled.
+    const uint8_t *const my_scales = lds + L::kScales + (wn * 32u * NT + col) * 16u;
+    auto store_scales = [&](const Metas &m, uint32_t chunk) {
+        uint8_t *const my_scales = lds + L::kScales + (wn * 32u * NT + (lane_number() & 31u)) * 16u;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (uint32_t j = 0; j < kMetas / 2u; ++j) reinterpret_cast<uint32_t *>(my_scales + (chunk & 1u) * L::kOuts * 16u + i * 512u)[j] = m.v[i][j];
+    };
+    auto scale_at = [&](uint32_t chunk, int i, uint32_t c) {
+        return meta_f32(*reinterpret_cast<const uint16_t *>(my_scales + (chunk & 1u) * L::kOuts * 16u + i * 512u + 2u * (GROUP == 128 ? c / 2u : c)), a.meta);
+    };
+
+    f32x16 acc[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            acc[m][i] = affine4_zero();
+            asm volatile("" : "+v"(acc[m][i]));
+        }
+    uint8_t *const sums = lds + L::kSum;
+    const uint32_t my_rows = wm * 32u * MT;  // the wave's first row of the tile
+    const uint8_t *const my_x = lds + (my_rows + col) * 128u;
+    auto read_x = [&](uint32_t place, uint32_t m, uint32_t j) {
+        const uint32_t piece = SUB32 ? 4u * (j / 2u) + 2u * half + j % 2u : 4u * half + j;
+        return *reinterpret_cast<const uint4 *>(my_x + place * L::kX + m * 4096u + ((piece ^ ((col >> 1) & 7u)) * 16u));
+    };
+    auto read_codes = [&](uint32_t from, uint32_t g, uint4 (&to)[NT]) {
+        const uint32_t l = lane_number(), c = l & 31u;  // (32 rows further on a quarter of the row's number is the same but for bits that are not looked at)
+        const uint8_t *const at = lds + L::kCodes + from * L::kB + (wn * 32u * NT + c) * 64u + (((2u * (g & 1u) + (l >> 5)) ^ ((c >> 2) & 3u)) * 16u);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) to[i] = *reinterpret_cast<const uint4 *>(at + i * 2048u);
+    };
+    // of groups of 32 lane half h has group h of the step: its halves to both (past the row's end there is no second group)
+    auto deal = [&](uint4 &v, uint32_t g) {
+        if constexpr (SUB32) {
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            if (64u * g + 32u >= a.k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = half ? 0u : w[j];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const auto q = __builtin_amdgcn_permlane32_swap(w[j], w[j + 2], false, false);
+                w[j] = q[0];
+                w[j + 2] = q[1];
+            }
+            v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    };
+    auto word = [](const uint4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; };
+    // The sums of step g's groups of the rows that are this wave's share.
+    auto form_sums = [&](uint32_t g, uint32_t place, uint32_t s, uint32_t chunk) {
+        const uint32_t l = lane_number(), col = l & 31u, half = l >> 5;
+        for (uint32_t m = wn; m < uint32_t(MT); m += WN) {
+            float sum[SUB32 ? 2 : 1] = {};
+            const uint8_t *const from = lds + place * L::kX + (my_rows + 32u * m + col) * 128u;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint32_t piece = SUB32 ? 4u * (j / 2u) + 2u * half + j % 2u : 4u * half + j;
+                sum[SUB32 ? j / 2u : 0u] = affine4_add<XT>(*reinterpret_cast<const uint4 *>(from + ((piece ^ ((col >> 1) & 7u)) * 16u)), sum[SUB32 ? j / 2u : 0u]);
+            }
+#pragma unroll
+            for (uint32_t c = 0; c < (SUB32 ? 2u : 1u); ++c) {
+                float v = add_xor32(sum[c]);
+                if (SUB32 && c == 1 && 64u * g + 32u >= a.k) v = 0.0f;
+                uint32_t terms[3];
+                bf16_terms(v, 0.0f, terms);
+                uint16_t *to = reinterpret_cast<uint16_t *>(sums + (chunk & 1u) * L::kSums + (my_rows + 32u * m + col) * 48u) + (SUB32 ? 2u * s + c : s);
+                if (half == 0)
+#pragma unroll
+                    for (int j = 0; j < 3; ++j) to[8 * j] = uint16_t(terms[j]);
+            }
+        }
+    };
+    // Where the next step's rows and codes have landed for every wave and the places of this step's are free again: of what was asked for after
+    // them, the rows of P - 2 steps and codes at every odd one of these, all may still be on their way.
+    auto meet = [&](uint32_t g, uint32_t place, uint32_t unit, auto odd_, auto &&between) {
+        constexpr uint32_t S = decltype(odd_)::value, kBetween = P - 2u, kOdd = kBetween / 2u + (kBetween % 2u && S == 0 ? 1u : 0u);
+        if (g + 2u * L::kUnits >= steps) wait_loads_and_sync<0>();
+        else wait_loads_and_sync<int(kBetween) * L::kLoadsX + int(kOdd) * L::kLoadsB>();
+        between();
+        if (S && g + 2u * L::kUnits - 1u < steps) load_b(unit, (g >> 1) + L::kUnits);
+        if (g + P < steps) load_x(place, g + P);
+    };
+    // Step g, the s-th of its chunk: a chain of kPer instructions a block (and group of 32). Between a chain's instructions stand the scaling of the
+    // chain before, the reads of the rows that come next into registers whose last use was the instruction ahead, and with the last
+    // rows' chains the unpacking of the next step's codes.
+    constexpr int kPer = SUB32 ? 2 : 4, kSubs = 4 / kPer;
+    Affine4Frag f[NT][4], xf[4];
+    uint4 raw[NT];
+    constexpr bool kBehind = NT == 1;
+    f32x16 p[kBehind ? 2 : 1];
+    float before = 0.0f;
+    auto step = [&](uint32_t g, uint32_t place, uint32_t next_place, uint32_t unit, uint32_t next_unit, uint32_t s, auto odd_, uint32_t chunk, auto &&between) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (m == 1) form_sums(g, place, s, chunk);
+            if (m == MT - 1 && g + 1u < steps) {
+                meet(g, place, unit, odd_, between);
+                read_codes(next_unit, g + 1u, raw);
+            }
+#pragma unroll
+            for (int c = 0; c < kSubs; ++c)
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const int chain = (m * kSubs + c) * NT + i, last = (chain + MT * kSubs * NT - 1) % (MT * kSubs * NT);  // the one before
+                    f32x16 &now = p[kBehind ? chain & 1 : 0], &old = p[kBehind ? (chain & 1) ^ 1 : 0];
+                    f32x16 &into = acc[last / NT / kSubs][last % NT];
+                    const float factor = before;
+                    before = scale_at(chunk, i, SUB32 ? 2u * s + c : s);
+                    if (m == MT - 1 && c == 0) deal(raw[i], g + 1u);
+#pragma unroll
+                    for (int j = c * kPer; j < c * kPer + kPer; ++j) {
+                        now = affine4_multiply<XT>(xf[j], f[i][j], j == c * kPer ? affine4_zero() : now);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (i == NT - 1) xf[j].v = m + 1 < MT ? read_x(place, m + 1u, j) : read_x(next_place, 0u, j);
+                        if (m == MT - 1) f[i][j] = affine4_codes<XT>(word(raw[i], j));
+                        constexpr int kEach = 16 / kPer;
+                        if (kBehind) {
+#pragma unroll
+                            for (int r = (j - c * kPer) * kEach; r < (j - c * kPer + 1) * kEach; ++r) into[r] = fmaf(factor, old[r], into[r]);
+                            asm volatile("" : "+v"(into));
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    if (!kBehind) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[m][i][r] = fmaf(before, now[r], acc[m][i][r]);
+                        asm volatile("" : "+v"(acc[m][i]));
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+        }
+    };
+    static_assert(MT * kSubs * NT % 2 == 0, "the chains alternate between two sums across steps");
+    // what no chain of a last chunk has written
+    auto clear_sums = [&](uint32_t chunk, uint32_t chains) {
+        for (uint32_t m = wn; m < uint32_t(MT); m += WN)
+            for (uint32_t c = chains; c < 8u && half == 0; ++c)
+#pragma unroll
+                for (int j = 0; j < 3; ++j) reinterpret_cast<uint16_t *>(sums + (chunk & 1u) * L::kSums + (my_rows + 32u * m + col) * 48u)[8 * j + c] = 0;
+    };
+    // The bias term of a chunk of `chains` chains: the lanes of half 0 add the sums' high terms, those of half 1 the middle ones, then half 0 the
+    // low ones, each against the (high) bias; an fp16 bias is two bf16 terms.
+    auto add_bias = [&](const Metas &bias, uint32_t chunk, uint32_t chains) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const float factor = a.biases ? 1.0f : -8.0f;
+            Affine4Frag high, low;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                uint32_t terms[3];
+                bf16_terms(2u * j < chains ? meta_at(bias, i, 2u * j) * factor : 0.0f, 2u * j + 1u < chains ? meta_at(bias, i, 2u * j + 1u) * factor : 0.0f, terms);
+                high.u[j] = terms[0];
+                low.u[j] = terms[1];
+            }
+            const uint32_t l = lane_number(), col = l & 31u, half = l >> 5;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const uint8_t *at = sums + (chunk & 1u) * L::kSums + (my_rows + 32u * m + col) * 48u;
+                Affine4Frag both, rest;
+                both.v = *reinterpret_cast<const uint4 *>(at + 16u * half);
+                rest.v = *reinterpret_cast<const uint4 *>(at + 32u);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) rest.u[j] = half ? 0u : rest.u[j];
+                f32x16 q = NT == 1 ? affine4_zero() : acc[m][i];
+                q = __builtin_amdgcn_mfma_f32_32x32x16_bf16(both.b, high.b, q, 0, 0, 0);
+                q = __builtin_amdgcn_mfma_f32_32x32x16_bf16(rest.b, high.b, q, 0, 0, 0);
+                if (a.meta == SHRIKE_META_F16) q = __builtin_amdgcn_mfma_f32_32x32x16_bf16(both.b, low.b, q, 0, 0, 0);
+                if (NT == 1)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) q[r] = __fadd_rn(acc[m][i][r], q[r]);
+                acc[m][i] = q;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+
+    Metas other;  // the next chunk's scales, or the last one's biases
+    // as if steps -P ... -1 had asked for them
+    load_b(0, 0);
+#pragma unroll
+    for (int v = 0; v < P; ++v) {
+        constexpr int kAhead = P % 2;  // v - P is odd where v is of the other parity than P
+        const uint32_t u = uint32_t((v - P - 1) / 2 + int(L::kUnits));
+        if (v % 2 != kAhead && u != 0u && 2u * u < steps) load_b(u, u);
+        if (uint32_t(v) < steps) load_x(v, v);
+    }
+    load_metas(other, scales, 0);
+    store_scales(other, 0);
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), in the compiler's own count
+    wait_loads_and_sync<0>();
+#pragma unroll
+    for (int r = 0; kBehind && r < 16; ++r) p[kBehind][r] = 0.0f;
+    auto begin = [&](uint32_t place, uint32_t unit, uint32_t g) {
+        read_codes(unit, g, raw);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            deal(raw[i], g);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[i][j] = affine4_codes<XT>(word(raw[i], j));
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) xf[j].v = read_x(place, 0, j);
+    };
+    begin(0, 0, 0);
+    uint32_t place = 0, unit = 0;
+    for (uint32_t chunk = 0; chunk < chunks; ++chunk) {
+        // The lane's own loads are waited for by the compiler, which knows nothing of the others on their way and waits for all: that is at the
+        // meetings, where the last of these were asked for a step ago and no new ones are yet.
+        auto one = [&](uint32_t s, auto odd_, auto &&between) {
+            const uint32_t g = chunk * kSteps + s, next_place = place == P - 1u ? 0u : place + 1u;
+            const uint32_t next_unit = !decltype(odd_)::value ? unit : unit == L::kUnits - 1u ? 0u : unit + 1u;
+            step(g, place, next_place, unit, next_unit, s, odd_, chunk, between);
+            place = next_place;
+            unit = next_unit;
+        };
+        const auto even = std::integral_constant<uint32_t, 0>{};
+        const auto odd = std::integral_constant<uint32_t, 1>{};
+        auto touch = [&] {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (uint32_t j = 0; j < kMetas / 2u; ++j) asm volatile("" : "+v"(other.v[i][j]));
+        };
+        one(0, even, [&] { load_metas(other, scales, chunk + 1u); });
+        if (chunk * kSteps + 1u < steps)
+            one(1, odd, [&] {
+                store_scales(other, chunk + 1u);
+                load_metas(other, biases, chunk);
+            });
+#pragma unroll 1
+        for (uint32_t s = 2; s < kSteps && chunk * kSteps + s < steps; s += 2u) {
+            one(s, even, [] {});
+            if (chunk * kSteps + s + 1u < steps) one(s + 1u, odd, [&] { if (s + 2u == kSteps) touch(); });
+        }
+        if (chunk * kSteps + 2u >= steps) load_metas(other, biases, chunk);  // (it had no second meeting)
+        // the chunk's bias term, once every wave has formed its sums
+        const uint32_t chains = min(8u, SUB32 ? groups - chunk * 8u : steps - chunk * kSteps);
+        if (chains < 8u) clear_sums(chunk, chains);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        add_bias(other, chunk, chains);
+        begin(place, unit, (chunk + 1u) * kSteps);  // (held across the bias term, the operands are spilled)
+    }
+#pragma unroll
+    for (int r = 0; kBehind && r < 16; ++r) acc[MT - 1][NT - 1][r] = fmaf(before, p[kBehind][r], acc[MT - 1][NT - 1][r]);
+    __syncthreads();
+    if (!active) return;
+
+    // ---- out: a block of 32 rows at a time through the wave's own part of LDS, so that a row's outputs leave 16 bytes a lane
+    const uint32_t size = a.out_type == SHRIKE_ELEM_F32 ? 4u : 2u, pitch = 32u * NT * size + 16u, outs = min(32u * NT, a.n - n_first);
+    uint8_t *const stage = lds + wave * 32u * (32u * NT * 4u + 16u);
+    const bool whole = (reinterpret_cast<uintptr_t>(a.out) | (a.out_stride * size)) % 16u == 0;
+    float extra[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) extra[i] = a.bias ? meta_f32(a.bias[min(n_first + 32u * i + col, a.n - 1u)], a.meta) : 0.0f;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        if (my_rows + 32u * m >= rows) break;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (uint32_t r = 0; r < 16; ++r) {
+                const float v = __fadd_rn(acc[m][i][r], extra[i]);
+                uint8_t *to = stage + (8u * (r / 4u) + 4u * half + r % 4u) * pitch + (32u * i + col) * size;
+                if (size == 4u) *reinterpret_cast<float *>(to) = v;
+                else *reinterpret_cast<uint16_t *>(to) = a.out_type == SHRIKE_ELEM_F16 ? f32_to_f16(v) : uint16_t(bf16_pair(v, 0.0f));
+            }
+        __builtin_amdgcn_wave_barrier();
+        const uint32_t per = 32u * NT * size / 16u;  // lanes a row
+        for (uint32_t at = lane; at < 32u * per; at += 64u) {
+            const uint32_t r = at / per, first = (at % per) * (16u / size), row = my_rows + 32u * m + r;
+            if (row >= rows || first >= outs) continue;
+            const uint8_t *from = stage + r * pitch + first * size;
+            uint8_t *to = static_cast<uint8_t *>(a.out) + (uint64_t(row0 + row) * a.out_stride + n_first + first) * size;
+            if (whole && first + 16u / size <= outs) {
+                *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(from);
+            } else {
+                for (uint32_t j = 0; j < 16u / size && first + j < outs; ++j) {
+                    if (size == 4u) reinterpret_cast<uint32_t *>(to)[j] = reinterpret_cast<const uint32_t *>(from)[j];
+                    else reinterpret_cast<uint16_t *>(to)[j] = reinterpret_cast<const uint16_t *>(from)[j];
+                }
+            }
+        }
+    }
+}
+
+template <int XT, int GROUP, int MT, int NT, int WM, int WN, int P>
+static int launch_tile(const Affine4Args &a, hipStream_t s) {
+    typedef TileLds<MT, NT, WM, WN, P> L;
+    hipLaunchKernelGGL((k_affine4_tile<XT, GROUP, MT, NT, WM, WN, P>), dim3((a.n + L::kOuts - 1u) / L::kOuts, (a.rows + L::kRows - 1u) / L::kRows),
+                       dim3(64u * L::kWaves), L::kBytes, s, a);
+    SHRIKE_HIP(hipGetLastError());
+    return 0;
+}
+
 template <int XT, int GROUP>
 static int launch_affine4(const Affine4Args &a, hipStream_t s) {
     if (a.rows <= 8u) return launch_few<XT, GROUP, 1>(a, s);
+    if (a.rows > 64u && a.x_stride * 512u < uint64_t(1) << 32) {  // (a tile's rows are reached by 32 bits)
+        if (uint64_t((a.n + 255u) / 256u) * ((a.rows + 255u) / 256u) >= 200u) return launch_tile<XT, GROUP, 4, 2, 2, 4, 3>(a, s);
+        if (uint64_t((a.n + 127u) / 128u) * ((a.rows + 127u) / 128u) >= 200u) return launch_tile<XT, GROUP, 4, 1, 1, 4, 6>(a, s);
+        return launch_tile<XT, GROUP, 2, 1, 1, 4, 6>(a, s);
+    }
     const uint64_t blocks = (a.n + 31u) / 32u;
     if (a.rows <= 16u || blocks * ((a.rows + 31u) / 32u) < 512u) return launch_few<XT, GROUP, 2>(a, s);
     return launch_few<XT, GROUP, 4>(a, s);
