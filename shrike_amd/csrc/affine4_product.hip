@@ -11,6 +11,7 @@
 #include "prefill_common.h"
 
 #include <type_traits>
+#include <utility>
 
 namespace shrike {
 
@@ -389,6 +390,17 @@ static int launch_few(const Affine4Args &args, hipStream_t s) {
 // two steps ahead in three places, two steps of the codes (64 bytes a row) in two. A chunk is eight chains (a chain is a group's products, or
 // half a group's of 128): its scales are a lane's own loads, a chunk ahead, and the bias term is added a chunk behind from the sums of the rows' groups,
 // which the waves form from the operands that they hold, WN waves a share of the tile's rows each.
+// Four bytes a lane into LDS, as lds_load16
+__device__ __forceinline__ void lds_load4(uint32_t lds, const void *base, uint32_t offset) {
+    const void *moved;
+    asm volatile("s_mov_b64 %0, %3\n\tglobal_load_lds_dword %2, %0" : "=&s"(moved) : "{m0}"(lds), "v"(offset), "s"(base) : "memory");
+}
+
+template <class Call, int... I>
+__device__ __forceinline__ void each_of(Call &&call, std::integer_sequence<int, I...>) {
+    (call(std::integral_constant<int, I>{}), ...);
+}
+
 // The lane's number, new at every call
 __device__ __forceinline__ uint32_t lane_number() {
     uint32_t l;
@@ -403,7 +415,9 @@ struct TileLds {
     static constexpr uint32_t kB = kOuts * 64u;     // two steps' codes
     static constexpr uint32_t kSums = kRows * 48u;  // a chunk's sums, three bf16 terms each
     static constexpr uint32_t kUnits = (P + 2u) / 2u;  // places of the codes: what is asked for beside a step is needed after its rows
-    static constexpr uint32_t kCodes = P * kX, kSum = kCodes + kUnits * kB, kScales = kSum + 2u * kSums, kBytes = kScales + 2u * kOuts * 16u;
+    static constexpr uint32_t kCodes = P * kX, kSum = kCodes + kUnits * kB, kScales = kSum + kSums;
+    // a chunk's scales (or biases) of 64 outputs, a word of each at a time: up to eight, that may start in the middle of a word
+    static constexpr uint32_t kMeta = 5u * 256u, kBiases = kScales + 2u * WN * kMeta, kBytes = kBiases + WN * kMeta;
     static constexpr int kLoadsX = int(kX / 1024u / kWaves), kLoadsB = int(kB / 1024u / kWaves);  // of a wave, a step (two steps)
     static_assert(kLoadsX * 1024u * kWaves == kX && kLoadsB * 1024u * kWaves == kB && kBytes <= 160u * 1024u);
     static_assert(kWaves * 32u * (32u * NT * 4u + 16u) <= kBytes, "the outputs on their way out fit");
@@ -458,55 +472,49 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
         }
     };
 
-    // ---- a chunk's scales and biases of the lane's outputs
+    // ---- a chunk's scales, a chunk ahead, and its biases, of the wave's outputs, a lane each: a run of 16-bit values that starts at any of them,
+    // so the words that it lies in, none past the tensor's last one. Waves of the same outputs share them out (one asks for scales, one for biases).
     const uint32_t n_first = n0 + wn * 32u * NT;
     const bool active = n_first < a.n;
     const uint32_t n_base = min(n_first, a.n - 1u);
-    const buffer_t scales = affine4_buffer(a.scales, uint64_t(n_base) * groups * 2u, uint64_t(a.n) * groups * 2u);
-    const buffer_t biases = a.biases ? affine4_buffer(a.biases, uint64_t(n_base) * groups * 2u, uint64_t(a.n) * groups * 2u) : scales;
-    struct Metas {
-        uint32_t v[NT][kMetas / 2];
+    constexpr uint32_t kWords = kMetas / 2u + 1u;
+    constexpr int kMetaLoads = int(kWords) * (WM == 1 ? 2 : 1);  // of a wave, a chunk
+    struct Run {
+        const uint8_t *from;  // the word that the wave's first output's values start in
+        uint32_t skew, last;  // where in it, and how far the tensor's last word lies from it, in bytes
     };
-    auto load_metas = [&](Metas &m, buffer_t from, uint32_t chunk) {
-        const uint32_t g = chunk * kMetas, l = lane_number() & 31u;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const uint32_t at = (min(n_first + 32u * i + l, a.n - 1u) - n_base) * groups * 2u;
-            if (g + kMetas > groups) {
-#pragma unroll
-                for (uint32_t j = 0; j < kMetas; ++j) {
-                    const uint32_t v = __builtin_amdgcn_raw_buffer_load_b16(from, at, min(g + j, groups - 1u) * 2u, 0);
-                    m.v[i][j / 2u] = j % 2u ? m.v[i][j / 2u] | v << 16 : v;
-                }
-            } else if constexpr (kMetas == 8u) {
-                const uint4 v = affine4_load16(from, at, g * 2u);
-                m.v[i][0] = v.x;
-                m.v[i][1] = v.y;
-                m.v[i][2] = v.z;
-                m.v[i][3] = v.w;
-            } else {
-                const auto v = __builtin_amdgcn_raw_buffer_load_b64(from, at, g * 2u, 0);
-                m.v[i][0] = v[0];
-                m.v[i][1] = v[1];
-            }
-        }
+    auto run_of = [&](const uint16_t *tensor) {
+        const uint8_t *const first = reinterpret_cast<const uint8_t *>(tensor + uint64_t(n_base) * groups);
+        Run r;
+        r.skew = uint32_t(reinterpret_cast<uintptr_t>(first) & 2u);
+        r.from = first - r.skew;
+        const uint64_t left = uint64_t(a.n - n_base) * groups * 2u + r.skew - 2u;
+        r.last = uint32_t(left < 0x7ffffffcull ? left : 0x7ffffffcull) & ~3u;
+        return r;
     };
-    // of chain c of the chunk
-    auto meta_at = [&](const Metas &m, int i, uint32_t c) {
-        const uint32_t j = GROUP == 128 ? c / 2u : c;
-        return meta_f32(uint16_t(m.v[i][j / 2u] >> 16u * (j % 2u)), a.meta);
-    };
-    // A chunk's scales wait in LDS, where the lane that wrote them reads them (both halves write the same): in registers something else is spilled.
-    const uint8_t *const my_scales = lds + L::kScales + (wn * 32u * NT + col) * 16u;
-    auto store_scales = [&](const Metas &m, uint32_t chunk) {
-        uint8_t *const my_scales = lds + L::kScales + (wn * 32u * NT + (lane_number() & 31u)) * 16u;
+    const Run scales = run_of(a.scales), biases = run_of(a.biases ? a.biases : a.scales);
+    // where the values of the lane's l-th output start, in bytes from `from` (a chunk's start is a whole number of words further on)
+    auto meta_start = [&](const Run &r, uint32_t l) { return r.skew + (min(n_first + l, a.n - 1u) - n_base) * groups * 2u; };
+    auto load_metas = [&](const Run &r, uint32_t to, uint32_t chunk) {
+        const uint32_t at = (meta_start(r, lane_number()) & ~3u) + chunk * kMetas * 2u;
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (uint32_t j = 0; j < kMetas / 2u; ++j) reinterpret_cast<uint32_t *>(my_scales + (chunk & 1u) * L::kOuts * 16u + i * 512u)[j] = m.v[i][j];
+        for (uint32_t j = 0; j < kWords; ++j) lds_load4(lds0 + to + j * 256u, r.from, min(at + 4u * j, r.last));
     };
+    auto load_both = [&](uint32_t chunk) {  // the next chunk's scales, this one's biases
+        if (WM == 1 || wm == 0) load_metas(scales, L::kScales + (((chunk + 1u) & 1u) * WN + wn) * L::kMeta, chunk + 1u);
+        if (WM == 1 || wm == 1) load_metas(biases, L::kBiases + wn * L::kMeta, chunk);
+    };
+    // a lane's scale of its i-th output and the chunk's chain c, an even or odd one of the chunk's scales
+    uint32_t scale_from[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const uint32_t l = 32u * i + col;
+        scale_from[i] = L::kScales + wn * L::kMeta + 4u * l + (meta_start(scales, l) & 2u);
+    }
     auto scale_at = [&](uint32_t chunk, int i, uint32_t c) {
-        return meta_f32(*reinterpret_cast<const uint16_t *>(my_scales + (chunk & 1u) * L::kOuts * 16u + i * 512u + 2u * (GROUP == 128 ? c / 2u : c)), a.meta);
+        const uint32_t e = GROUP == 128 ? c / 2u : c, into = scale_from[i] & 2u;
+        const uint32_t odd = e % 2u ? (into ? 254u : 2u) : 0u;
+        return *reinterpret_cast<const uint16_t *>(lds + (chunk & 1u) * (WN * L::kMeta) + scale_from[i] + odd + e / 2u * 256u);
     };
 
     f32x16 acc[MT][NT];
@@ -517,6 +525,7 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
             acc[m][i] = affine4_zero();
             asm volatile("" : "+v"(acc[m][i]));
         }
+    constexpr int kPer = SUB32 ? 2 : 4, kSubs = 4 / kPer;  // instructions a chain, chains a block and step
     uint8_t *const sums = lds + L::kSum;
     const uint32_t my_rows = wm * 32u * MT;  // the wave's first row of the tile
     const uint8_t *const my_x = lds + (my_rows + col) * 128u;
@@ -547,116 +556,136 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
         }
     };
     auto word = [](const uint4 &v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; };
-    // The sums of step g's groups of the rows that are this wave's share.
-    auto form_sums = [&](uint32_t g, uint32_t place, uint32_t s, uint32_t chunk) {
-        const uint32_t l = lane_number(), col = l & 31u, half = l >> 5;
-        for (uint32_t m = wn; m < uint32_t(MT); m += WN) {
-            float sum[SUB32 ? 2 : 1] = {};
-            const uint8_t *const from = lds + place * L::kX + (my_rows + 32u * m + col) * 128u;
+    // The sums of a step's groups of the rows that are this wave's share: its pieces are read, added and written a few instructions a slot.
+    static_assert(MT <= WN && MT * NT >= 2, "a wave has a share of 32 rows at most, and the reads stand ahead of the meeting");
+    const uint32_t share = min(wn, uint32_t(MT - 1));
+    uint4 sum_piece[2];
+    float sum_of[kSubs];
+    auto form_sums = [&](auto slot_, uint32_t g, uint32_t place, uint32_t s) {
+        constexpr int slot = decltype(slot_)::value;
+        if constexpr (slot >= 2 && slot < 6) {
+            constexpr int j = slot - 2, c = j / kPer;
+            sum_of[c] = affine4_add<XT>(sum_piece[j % 2], j % kPer ? sum_of[c] : 0.0f);
+        }
+        if constexpr (slot < 4) {
+            const uint32_t l = lane_number(), col = l & 31u, half = l >> 5, piece = SUB32 ? 4u * (slot / 2u) + 2u * half + slot % 2u : 4u * half + slot;
+            sum_piece[slot % 2] = *reinterpret_cast<const uint4 *>(lds + place * L::kX + (my_rows + 32u * share + col) * 128u + ((piece ^ ((col >> 1) & 7u)) * 16u));
+        }
+        if constexpr (slot == 6) {
+            const uint32_t l = lane_number(), col = l & 31u, half = l >> 5;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
-                const uint32_t piece = SUB32 ? 4u * (j / 2u) + 2u * half + j % 2u : 4u * half + j;
-                sum[SUB32 ? j / 2u : 0u] = affine4_add<XT>(*reinterpret_cast<const uint4 *>(from + ((piece ^ ((col >> 1) & 7u)) * 16u)), sum[SUB32 ? j / 2u : 0u]);
-            }
-#pragma unroll
-            for (uint32_t c = 0; c < (SUB32 ? 2u : 1u); ++c) {
-                float v = add_xor32(sum[c]);
+            for (int c = 0; c < kSubs; ++c) {
+                float v = add_xor32(sum_of[c]);
                 if (SUB32 && c == 1 && 64u * g + 32u >= a.k) v = 0.0f;
                 uint32_t terms[3];
                 bf16_terms(v, 0.0f, terms);
-                uint16_t *to = reinterpret_cast<uint16_t *>(sums + (chunk & 1u) * L::kSums + (my_rows + 32u * m + col) * 48u) + (SUB32 ? 2u * s + c : s);
-                if (half == 0)
+                uint16_t *to = reinterpret_cast<uint16_t *>(sums + (my_rows + 32u * share + col) * 48u) + (SUB32 ? 2u * s + c : s);
+                if (half == 0 && wn < uint32_t(MT))
 #pragma unroll
                     for (int j = 0; j < 3; ++j) to[8 * j] = uint16_t(terms[j]);
             }
         }
     };
     // Where the next step's rows and codes have landed for every wave and the places of this step's are free again: of what was asked for after
-    // them, the rows of P - 2 steps and codes at every odd one of these, all may still be on their way.
-    auto meet = [&](uint32_t g, uint32_t place, uint32_t unit, auto odd_, auto &&between) {
+    // them, the rows of P - 2 steps, codes at every odd one of these and a chunk's scales and biases at its first, all may still be on their way.
+    auto meet = [&](uint32_t g, uint32_t place, uint32_t unit, uint32_t s, auto odd_, uint32_t chunk) {
         constexpr uint32_t S = decltype(odd_)::value, kBetween = P - 2u, kOdd = kBetween / 2u + (kBetween % 2u && S == 0 ? 1u : 0u);
         if (g + 2u * L::kUnits >= steps) wait_loads_and_sync<0>();
+        else if (s >= 1u && s <= kBetween) wait_loads_and_sync<int(kBetween) * L::kLoadsX + int(kOdd) * L::kLoadsB + kMetaLoads>();
         else wait_loads_and_sync<int(kBetween) * L::kLoadsX + int(kOdd) * L::kLoadsB>();
-        between();
+        if (s == 0) load_both(chunk);
         if (S && g + 2u * L::kUnits - 1u < steps) load_b(unit, (g >> 1) + L::kUnits);
         if (g + P < steps) load_x(place, g + P);
     };
     // Step g, the s-th of its chunk: a chain of kPer instructions a block (and group of 32). Between a chain's instructions stand the scaling of the
     // chain before, the reads of the rows that come next into registers whose last use was the instruction ahead, and with the last
     // rows' chains the unpacking of the next step's codes.
-    constexpr int kPer = SUB32 ? 2 : 4, kSubs = 4 / kPer;
     Affine4Frag f[NT][4], xf[4];
     uint4 raw[NT];
     constexpr bool kBehind = NT == 1;
     f32x16 p[kBehind ? 2 : 1];
-    float before = 0.0f;
-    auto step = [&](uint32_t g, uint32_t place, uint32_t next_place, uint32_t unit, uint32_t next_unit, uint32_t s, auto odd_, uint32_t chunk, auto &&between) {
+    float before[2] = {0.0f, 0.0f};  // the scales of the chain before and of this one
+    uint16_t next_scale = 0;  // of the chain that comes next
+    auto step = [&](uint32_t g, uint32_t place, uint32_t next_place, uint32_t unit, uint32_t next_unit, uint32_t s, auto odd_, uint32_t chunk) {
+        const uint32_t scale_chunk = s + 1u == kSteps ? chunk + 1u : chunk, scale_step = s + 1u == kSteps ? 0u : s + 1u;  // the next step's
+        auto slots = [&](auto slot_) {  // an instruction and what stands behind it
+            constexpr int slot = decltype(slot_)::value, j = slot % kPer, chain = slot / kPer, i = chain % NT, c = chain / NT % kSubs, m = chain / NT / kSubs;
+            constexpr int chains = MT * kSubs * NT, last = (chain + chains - 1) % chains, next = (chain + 1) % chains, at = c * kPer + j;
+            f32x16 &now = p[kBehind ? chain & 1 : 0], &old = p[kBehind ? (chain & 1) ^ 1 : 0];
+            f32x16 &into = acc[last / NT / kSubs][last % NT];
+            if constexpr (j == 0) {
+                if constexpr (m == MT - 1 && c == 0 && i == 0) {
+                    meet(g, place, unit, s, odd_, chunk);
+                    read_codes(next_unit, g + 1u, raw);  // (behind the last step: something)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            if (m == 1) form_sums(g, place, s, chunk);
-            if (m == MT - 1 && g + 1u < steps) {
-                meet(g, place, unit, odd_, between);
-                read_codes(next_unit, g + 1u, raw);
-            }
-#pragma unroll
-            for (int c = 0; c < kSubs; ++c)
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    const int chain = (m * kSubs + c) * NT + i, last = (chain + MT * kSubs * NT - 1) % (MT * kSubs * NT);  // the one before
-                    f32x16 &now = p[kBehind ? chain & 1 : 0], &old = p[kBehind ? (chain & 1) ^ 1 : 0];
-                    f32x16 &into = acc[last / NT / kSubs][last % NT];
-                    const float factor = before;
-                    before = scale_at(chunk, i, SUB32 ? 2u * s + c : s);
-                    if (m == MT - 1 && c == 0) deal(raw[i], g + 1u);
-#pragma unroll
-                    for (int j = c * kPer; j < c * kPer + kPer; ++j) {
-                        now = affine4_multiply<XT>(xf[j], f[i][j], j == c * kPer ? affine4_zero() : now);
-                        __builtin_amdgcn_sched_barrier(0);
-                        if (i == NT - 1) xf[j].v = m + 1 < MT ? read_x(place, m + 1u, j) : read_x(next_place, 0u, j);
-                        if (m == MT - 1) f[i][j] = affine4_codes<XT>(word(raw[i], j));
-                        constexpr int kEach = 16 / kPer;
-                        if (kBehind) {
-#pragma unroll
-                            for (int r = (j - c * kPer) * kEach; r < (j - c * kPer + 1) * kEach; ++r) into[r] = fmaf(factor, old[r], into[r]);
-                            asm volatile("" : "+v"(into));
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                    if (!kBehind) {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) acc[m][i][r] = fmaf(before, now[r], acc[m][i][r]);
-                        asm volatile("" : "+v"(acc[m][i]));
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
+                    for (int n = 0; n < NT; ++n) asm volatile("" : "+v"(raw[n].x), "+v"(raw[n].y), "+v"(raw[n].z), "+v"(raw[n].w));
                 }
-        }
+                if constexpr (m == MT - 1 && c == 0) deal(raw[i], g + 1u);
+                before[0] = before[1];
+                before[1] = meta_f32(next_scale, a.meta);
+            }
+            now = affine4_multiply<XT>(xf[at], f[i][at], j == 0 ? affine4_zero() : now);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (j == 0) next_scale = scale_at(next ? chunk : scale_chunk, next % NT, SUB32 ? 2u * (next ? s : scale_step) + next / NT % kSubs : next ? s : scale_step);
+            if constexpr (i == NT - 1) xf[at].v = m + 1 < MT ? read_x(place, m + 1u, at) : read_x(next_place, 0u, at);
+            if constexpr (m == MT - 1) {
+                f[i][at] = affine4_codes<XT>(word(raw[i], at));
+                asm volatile("" : "+v"(f[i][at].v.x), "+v"(f[i][at].v.y), "+v"(f[i][at].v.z), "+v"(f[i][at].v.w));  // (here: else it sinks behind the branches)
+            }
+            form_sums(slot_, g, place, s);
+            if constexpr (kBehind) {
+                constexpr int kEach = 16 / kPer;
+#pragma unroll
+                for (int r = j * kEach; r < (j + 1) * kEach; ++r) into[r] = fmaf(before[0], old[r], into[r]);
+                asm volatile("" : "+v"(into));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (!kBehind && j == kPer - 1) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[m][i][r] = fmaf(before[1], now[r], acc[m][i][r]);
+                asm volatile("" : "+v"(acc[m][i]));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        each_of(slots, std::make_integer_sequence<int, MT * NT * 4>{});
     };
     static_assert(MT * kSubs * NT % 2 == 0, "the chains alternate between two sums across steps");
     // what no chain of a last chunk has written
-    auto clear_sums = [&](uint32_t chunk, uint32_t chains) {
+    auto clear_sums = [&](uint32_t chains) {
         for (uint32_t m = wn; m < uint32_t(MT); m += WN)
             for (uint32_t c = chains; c < 8u && half == 0; ++c)
 #pragma unroll
-                for (int j = 0; j < 3; ++j) reinterpret_cast<uint16_t *>(sums + (chunk & 1u) * L::kSums + (my_rows + 32u * m + col) * 48u)[8 * j + c] = 0;
+                for (int j = 0; j < 3; ++j) reinterpret_cast<uint16_t *>(sums + (my_rows + 32u * m + col) * 48u)[8 * j + c] = 0;
     };
     // The bias term of a chunk of `chains` chains: the lanes of half 0 add the sums' high terms, those of half 1 the middle ones, then half 0 the
     // low ones, each against the (high) bias; an fp16 bias is two bf16 terms.
-    auto add_bias = [&](const Metas &bias, uint32_t chunk, uint32_t chains) {
+    auto add_bias = [&](uint32_t chains) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const float factor = a.biases ? 1.0f : -8.0f;
+            const uint32_t l = lane_number(), col = l & 31u, half = l >> 5;
+            // the run's words, brought to where it starts; of groups of 128 each value twice
+            const uint8_t *const run = lds + L::kBiases + wn * L::kMeta + 4u * (32u * i + col);
+            const uint32_t skew = 8u * (meta_start(biases, 32u * i + col) & 2u);
+            uint32_t words[kWords], pairs[4];
+#pragma unroll
+            for (uint32_t j = 0; j < kWords; ++j) words[j] = *reinterpret_cast<const uint32_t *>(run + j * 256u);
+#pragma unroll
+            for (uint32_t j = 0; j + 1u < kWords; ++j) words[j] = __builtin_amdgcn_alignbit(words[j + 1u], words[j], skew);
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) pairs[j] = GROUP == 128 ? (words[j / 2u] >> 16u * (j % 2u) & 0xffffu) * 0x10001u : words[j];
             Affine4Frag high, low;
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
                 uint32_t terms[3];
-                bf16_terms(2u * j < chains ? meta_at(bias, i, 2u * j) * factor : 0.0f, 2u * j + 1u < chains ? meta_at(bias, i, 2u * j + 1u) * factor : 0.0f, terms);
+                auto value = [&](uint32_t c) { return c < chains ? meta_f32(uint16_t(pairs[c / 2u] >> 16u * (c % 2u)), a.meta) * factor : 0.0f; };
+                bf16_terms(value(2u * j), value(2u * j + 1u), terms);
                 high.u[j] = terms[0];
                 low.u[j] = terms[1];
             }
-            const uint32_t l = lane_number(), col = l & 31u, half = l >> 5;
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                const uint8_t *at = sums + (chunk & 1u) * L::kSums + (my_rows + 32u * m + col) * 48u;
+                const uint8_t *at = sums + (my_rows + 32u * m + col) * 48u;
                 Affine4Frag both, rest;
                 both.v = *reinterpret_cast<const uint4 *>(at + 16u * half);
                 rest.v = *reinterpret_cast<const uint4 *>(at + 32u);
@@ -675,7 +704,7 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
         }
     };
 
-    Metas other;  // the next chunk's scales, or the last one's biases
+    if (WM == 1 || wm == 0) load_metas(scales, L::kScales + wn * L::kMeta, 0);
     // as if steps -P ... -1 had asked for them
     load_b(0, 0);
 #pragma unroll
@@ -685,9 +714,6 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
         if (v % 2 != kAhead && u != 0u && 2u * u < steps) load_b(u, u);
         if (uint32_t(v) < steps) load_x(v, v);
     }
-    load_metas(other, scales, 0);
-    store_scales(other, 0);
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), in the compiler's own count
     wait_loads_and_sync<0>();
 #pragma unroll
     for (int r = 0; kBehind && r < 16; ++r) p[kBehind][r] = 0.0f;
@@ -703,46 +729,32 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
         for (uint32_t j = 0; j < 4; ++j) xf[j].v = read_x(place, 0, j);
     };
     begin(0, 0, 0);
+    next_scale = scale_at(0, 0, 0);
     uint32_t place = 0, unit = 0;
     for (uint32_t chunk = 0; chunk < chunks; ++chunk) {
-        // The lane's own loads are waited for by the compiler, which knows nothing of the others on their way and waits for all: that is at the
-        // meetings, where the last of these were asked for a step ago and no new ones are yet.
-        auto one = [&](uint32_t s, auto odd_, auto &&between) {
+        auto one = [&](uint32_t s, auto odd_) {
             const uint32_t g = chunk * kSteps + s, next_place = place == P - 1u ? 0u : place + 1u;
             const uint32_t next_unit = !decltype(odd_)::value ? unit : unit == L::kUnits - 1u ? 0u : unit + 1u;
-            step(g, place, next_place, unit, next_unit, s, odd_, chunk, between);
+            step(g, place, next_place, unit, next_unit, s, odd_, chunk);
             place = next_place;
             unit = next_unit;
         };
-        const auto even = std::integral_constant<uint32_t, 0>{};
-        const auto odd = std::integral_constant<uint32_t, 1>{};
-        auto touch = [&] {
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (uint32_t j = 0; j < kMetas / 2u; ++j) asm volatile("" : "+v"(other.v[i][j]));
-        };
-        one(0, even, [&] { load_metas(other, scales, chunk + 1u); });
-        if (chunk * kSteps + 1u < steps)
-            one(1, odd, [&] {
-                store_scales(other, chunk + 1u);
-                load_metas(other, biases, chunk);
-            });
 #pragma unroll 1
-        for (uint32_t s = 2; s < kSteps && chunk * kSteps + s < steps; s += 2u) {
-            one(s, even, [] {});
-            if (chunk * kSteps + s + 1u < steps) one(s + 1u, odd, [&] { if (s + 2u == kSteps) touch(); });
+        for (uint32_t s = 0; s < kSteps && chunk * kSteps + s < steps; s += 2u) {
+            one(s, std::integral_constant<uint32_t, 0>{});
+            if (chunk * kSteps + s + 1u < steps) one(s + 1u, std::integral_constant<uint32_t, 1>{});
         }
-        if (chunk * kSteps + 2u >= steps) load_metas(other, biases, chunk);  // (it had no second meeting)
         // the chunk's bias term, once every wave has formed its sums
         const uint32_t chains = min(8u, SUB32 ? groups - chunk * 8u : steps - chunk * kSteps);
-        if (chains < 8u) clear_sums(chunk, chains);
+        if (chains < 8u) clear_sums(chains);
+        if (chunk + 1u == chunks) wait_loads_and_sync<0>();
+        else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        add_bias(chains);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        add_bias(other, chunk, chains);
         begin(place, unit, (chunk + 1u) * kSteps);  // (held across the bias term, the operands are spilled)
     }
 #pragma unroll
-    for (int r = 0; kBehind && r < 16; ++r) acc[MT - 1][NT - 1][r] = fmaf(before, p[kBehind][r], acc[MT - 1][NT - 1][r]);
+    for (int r = 0; kBehind && r < 16; ++r) acc[MT - 1][NT - 1][r] = fmaf(before[1], p[kBehind][r], acc[MT - 1][NT - 1][r]);
     __syncthreads();
     if (!active) return;
 
@@ -799,8 +811,8 @@ static int launch_affine4(const Affine4Args &a, hipStream_t s) {
     if (a.rows <= 8u) return launch_few<XT, GROUP, 1>(a, s);
     if (a.rows > 64u && a.x_stride * 512u < uint64_t(1) << 32) {  // (a tile's rows are reached by 32 bits)
         if (uint64_t((a.n + 255u) / 256u) * ((a.rows + 255u) / 256u) >= 200u) return launch_tile<XT, GROUP, 4, 2, 2, 4, 3>(a, s);
-        if (uint64_t((a.n + 127u) / 128u) * ((a.rows + 127u) / 128u) >= 200u) return launch_tile<XT, GROUP, 4, 1, 1, 4, 6>(a, s);
-        return launch_tile<XT, GROUP, 2, 1, 1, 4, 6>(a, s);
+        if (uint64_t((a.n + 127u) / 128u) * ((a.rows + 127u) / 128u) >= 512u) return launch_tile<XT, GROUP, 4, 1, 1, 4, 3>(a, s);
+        return launch_tile<XT, GROUP, 2, 1, 1, 4, 4>(a, s);
     }
     const uint64_t blocks = (a.n + 31u) / 32u;
     if (a.rows <= 16u || blocks * ((a.rows + 31u) / 32u) < 512u) return launch_few<XT, GROUP, 2>(a, s);
