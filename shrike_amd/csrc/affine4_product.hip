@@ -408,7 +408,7 @@ __device__ __forceinline__ uint32_t lane_number() {
     return l;
 }
 
-template <int MT, int NT, int WM, int WN, int P>
+template <int MT, int NT, int WM, int WN, int P, int KS>
 struct TileLds {
     static constexpr uint32_t kRows = 32u * MT * WM, kOuts = 32u * NT * WN, kWaves = WM * WN;
     static constexpr uint32_t kX = kRows * 128u;    // a step's rows
@@ -416,31 +416,36 @@ struct TileLds {
     static constexpr uint32_t kSums = kRows * 48u;  // a chunk's sums, three bf16 terms each
     static constexpr uint32_t kUnits = (P + 2u) / 2u;  // places of the codes: what is asked for beside a step is needed after its rows
     static constexpr uint32_t kCodes = P * kX, kSum = kCodes + kUnits * kB, kScales = kSum + kSums;
-    // a chunk's scales (or biases) of 64 outputs, a word of each at a time: up to eight, that may start in the middle of a word
-    static constexpr uint32_t kMeta = 5u * 256u, kBiases = kScales + 2u * WN * kMeta, kBytes = kBiases + WN * kMeta;
+    // a chunk's scales (or biases) of a wave's outputs, a word of each at a time: up to eight, that may start in the middle of a word
+    static constexpr uint32_t kMeta = 5u * 128u * NT, kBiases = kScales + 2u * WN * kMeta, kBytes = (kBiases + WN * kMeta + 127u) & ~127u;
     static constexpr int kLoadsX = int(kX / 1024u / kWaves), kLoadsB = int(kB / 1024u / kWaves);  // of a wave, a step (two steps)
-    static_assert(kLoadsX * 1024u * kWaves == kX && kLoadsB * 1024u * kWaves == kB && kBytes <= 160u * 1024u);
-    static_assert(kWaves * 32u * (32u * NT * 4u + 16u) <= kBytes, "the outputs on their way out fit");
+    static_assert(kLoadsX * 1024u * kWaves == kX && kLoadsB * 1024u * kWaves == kB && KS * kBytes <= 160u * 1024u);
+    static_assert(kWaves * 32u * (32u * NT * 4u + 16u) <= kBytes && (KS == 1 || kWaves * MT * NT * 4096u <= kBytes), "the outputs on their way out fit, and a part's sums");
 };
 
-template <int XT, int GROUP, int MT, int NT, int WM, int WN, int P>
-__global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(Affine4Args a) {
-    typedef TileLds<MT, NT, WM, WN, P> L;
+template <int XT, int GROUP, int MT, int NT, int WM, int WN, int P, int KS>
+__global__ __launch_bounds__(64 * WM * WN * KS, 2) void k_affine4_tile(Affine4Args a) {
+    typedef TileLds<MT, NT, WM, WN, P, KS> L;
     constexpr bool SUB32 = GROUP == 32;
     constexpr uint32_t kSteps = SUB32 ? 4u : 8u;               // of a chunk
     constexpr uint32_t kMetas = GROUP == 128 ? 4u : 8u;        // a chunk's scales
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // (of a size that the compiler does not know: else it takes sums to the accumulation registers and back)
     const uint32_t lane = threadIdx.x & 63u, col = lane & 31u, half = lane >> 5;
-    const uint32_t wave = wave_index(), wm = wave / WN, wn = wave % WN;
-    const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)lds));
-    const uint32_t steps = (a.k + 63u) / 64u, chunks = (steps + kSteps - 1u) / kSteps, groups = a.k / uint32_t(GROUP);
+    // the workgroup's waves are KS parts of k, whole chunks each, with their own places in LDS
+    const uint32_t part = wave_index() / L::kWaves, wave = wave_index() % L::kWaves, wm = wave / WN, wn = wave % WN;
+    const uint32_t steps_in_all = (a.k + 63u) / 64u, chunks = ((steps_in_all + kSteps - 1u) / kSteps + KS - 1u) / KS;  // of a part, the first ones
+    const uint32_t first_step = min(part * chunks * kSteps, steps_in_all), steps = min(chunks * kSteps, steps_in_all - first_step);
+    const uint32_t my_k = steps ? a.k - first_step * 64u : 0u;  // what is left of a row where the part begins
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_of_parts[];  // (of a size that the compiler does not know: else it takes sums to the accumulation registers and back)
+    uint8_t *const lds = lds_of_parts + part * L::kBytes;
+    const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)lds_of_parts)) + part * L::kBytes;
+    const uint32_t groups = a.k / uint32_t(GROUP), my_groups = my_k / uint32_t(GROUP);
     const uint32_t row0 = blockIdx.y * L::kRows, n0 = blockIdx.x * L::kOuts, rows = min(a.rows - row0, L::kRows);
 
     // ---- what the wave asks for: eight rows of x a load (eight lanes a row, pieces xor-ed with half the row's number), sixteen of codes
     // (four lanes a row, xor-ed with a quarter of it). Rows and outputs past the last are the last again; past k stands a row's last piece.
-    const uint32_t pieces = a.k / 8u, code_pieces = a.k / 32u;
-    const uint8_t *const x = reinterpret_cast<const uint8_t *>(a.x + uint64_t(row0) * a.x_stride);
-    const uint8_t *const codes = a.codes + uint64_t(n0) * (a.k / 2u);
+    const uint32_t pieces = my_k / 8u, code_pieces = my_k / 32u;
+    const uint8_t *const x = reinterpret_cast<const uint8_t *>(a.x + uint64_t(row0) * a.x_stride) + first_step * 128u;
+    const uint8_t *const codes = a.codes + uint64_t(n0) * (a.k / 2u) + first_step * 32u;
     // (The offsets are formed again from the lane's number at every use: held in registers, they are spilled.)
     const uint32_t stride = uint32_t(a.x_stride) * 2u, row_bytes = a.k / 2u;
     auto load_x = [&](uint32_t place, uint32_t g) {
@@ -484,11 +489,11 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
         uint32_t skew, last;  // where in it, and how far the tensor's last word lies from it, in bytes
     };
     auto run_of = [&](const uint16_t *tensor) {
-        const uint8_t *const first = reinterpret_cast<const uint8_t *>(tensor + uint64_t(n_base) * groups);
+        const uint8_t *const first = reinterpret_cast<const uint8_t *>(tensor + uint64_t(n_base) * groups + (steps ? part * chunks * kMetas : 0u));
         Run r;
         r.skew = uint32_t(reinterpret_cast<uintptr_t>(first) & 2u);
         r.from = first - r.skew;
-        const uint64_t left = uint64_t(a.n - n_base) * groups * 2u + r.skew - 2u;
+        const uint64_t left = (uint64_t(a.n - n_base) * groups - (steps ? part * chunks * kMetas : 0u)) * 2u + r.skew - 2u;
         r.last = uint32_t(left < 0x7ffffffcull ? left : 0x7ffffffcull) & ~3u;
         return r;
     };
@@ -496,9 +501,10 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
     // where the values of the lane's l-th output start, in bytes from `from` (a chunk's start is a whole number of words further on)
     auto meta_start = [&](const Run &r, uint32_t l) { return r.skew + (min(n_first + l, a.n - 1u) - n_base) * groups * 2u; };
     auto load_metas = [&](const Run &r, uint32_t to, uint32_t chunk) {
-        const uint32_t at = (meta_start(r, lane_number()) & ~3u) + chunk * kMetas * 2u;
+        const uint32_t l = lane_number(), at = (meta_start(r, l) & ~3u) + chunk * kMetas * 2u;
+        if (NT == 2 || l < 32u)
 #pragma unroll
-        for (uint32_t j = 0; j < kWords; ++j) lds_load4(lds0 + to + j * 256u, r.from, min(at + 4u * j, r.last));
+        for (uint32_t j = 0; j < kWords; ++j) lds_load4(lds0 + to + j * (128u * NT), r.from, min(at + 4u * j, r.last));
     };
     auto load_both = [&](uint32_t chunk) {  // the next chunk's scales, this one's biases
         if (WM == 1 || wm == 0) load_metas(scales, L::kScales + (((chunk + 1u) & 1u) * WN + wn) * L::kMeta, chunk + 1u);
@@ -513,8 +519,8 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
     }
     auto scale_at = [&](uint32_t chunk, int i, uint32_t c) {
         const uint32_t e = GROUP == 128 ? c / 2u : c, into = scale_from[i] & 2u;
-        const uint32_t odd = e % 2u ? (into ? 254u : 2u) : 0u;
-        return *reinterpret_cast<const uint16_t *>(lds + (chunk & 1u) * (WN * L::kMeta) + scale_from[i] + odd + e / 2u * 256u);
+        const uint32_t odd = e % 2u ? (into ? 128u * NT - 2u : 2u) : 0u;
+        return *reinterpret_cast<const uint16_t *>(lds + (chunk & 1u) * (WN * L::kMeta) + scale_from[i] + odd + e / 2u * (128u * NT));
     };
 
     f32x16 acc[MT][NT];
@@ -543,7 +549,7 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
     auto deal = [&](uint4 &v, uint32_t g) {
         if constexpr (SUB32) {
             uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            if (64u * g + 32u >= a.k)
+            if (64u * g + 32u >= my_k)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) w[j] = half ? 0u : w[j];
 #pragma unroll
@@ -568,15 +574,14 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
             sum_of[c] = affine4_add<XT>(sum_piece[j % 2], j % kPer ? sum_of[c] : 0.0f);
         }
         if constexpr (slot < 4) {
-            const uint32_t l = lane_number(), col = l & 31u, half = l >> 5, piece = SUB32 ? 4u * (slot / 2u) + 2u * half + slot % 2u : 4u * half + slot;
-            sum_piece[slot % 2] = *reinterpret_cast<const uint4 *>(lds + place * L::kX + (my_rows + 32u * share + col) * 128u + ((piece ^ ((col >> 1) & 7u)) * 16u));
+            sum_piece[slot % 2] = read_x(place, share, slot);
         }
         if constexpr (slot == 6) {
             const uint32_t l = lane_number(), col = l & 31u, half = l >> 5;
 #pragma unroll
             for (int c = 0; c < kSubs; ++c) {
                 float v = add_xor32(sum_of[c]);
-                if (SUB32 && c == 1 && 64u * g + 32u >= a.k) v = 0.0f;
+                if (SUB32 && c == 1 && 64u * g + 32u >= my_k) v = 0.0f;
                 uint32_t terms[3];
                 bf16_terms(v, 0.0f, terms);
                 uint16_t *to = reinterpret_cast<uint16_t *>(sums + (my_rows + 32u * share + col) * 48u) + (SUB32 ? 2u * s + c : s);
@@ -602,12 +607,23 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
     // rows' chains the unpacking of the next step's codes.
     Affine4Frag f[NT][4], xf[4];
     uint4 raw[NT];
-    constexpr bool kBehind = NT == 1;
+    constexpr bool kBehind = NT == 1 || !SUB32;  // (else the second sum is spilled)
     f32x16 p[kBehind ? 2 : 1];
-    float before[2] = {0.0f, 0.0f};  // the scales of the chain before and of this one
-    uint16_t next_scale = 0;  // of the chain that comes next
+    float before = 0.0f;  // the scale of the step before's last chain
+    uint16_t next_scales[kSubs][NT];  // the next step's, as they are
+    float factors[kSubs][NT] = {};
+    auto read_scales = [&](uint32_t chunk, uint32_t s) {
+#pragma unroll
+        for (int c = 0; c < kSubs; ++c)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) next_scales[c][i] = scale_at(chunk, i, SUB32 ? 2u * s + c : s);
+    };
     auto step = [&](uint32_t g, uint32_t place, uint32_t next_place, uint32_t unit, uint32_t next_unit, uint32_t s, auto odd_, uint32_t chunk) {
-        const uint32_t scale_chunk = s + 1u == kSteps ? chunk + 1u : chunk, scale_step = s + 1u == kSteps ? 0u : s + 1u;  // the next step's
+        before = factors[kSubs - 1][NT - 1];
+#pragma unroll
+        for (int c = 0; c < kSubs; ++c)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) factors[c][i] = meta_f32(next_scales[c][i], a.meta);
         auto slots = [&](auto slot_) {  // an instruction and what stands behind it
             constexpr int slot = decltype(slot_)::value, j = slot % kPer, chain = slot / kPer, i = chain % NT, c = chain / NT % kSubs, m = chain / NT / kSubs;
             constexpr int chains = MT * kSubs * NT, last = (chain + chains - 1) % chains, next = (chain + 1) % chains, at = c * kPer + j;
@@ -621,12 +637,10 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
                     for (int n = 0; n < NT; ++n) asm volatile("" : "+v"(raw[n].x), "+v"(raw[n].y), "+v"(raw[n].z), "+v"(raw[n].w));
                 }
                 if constexpr (m == MT - 1 && c == 0) deal(raw[i], g + 1u);
-                before[0] = before[1];
-                before[1] = meta_f32(next_scale, a.meta);
             }
             now = affine4_multiply<XT>(xf[at], f[i][at], j == 0 ? affine4_zero() : now);
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (j == 0) next_scale = scale_at(next ? chunk : scale_chunk, next % NT, SUB32 ? 2u * (next ? s : scale_step) + next / NT % kSubs : next ? s : scale_step);
+            if constexpr (slot == 1) read_scales(s + 1u == kSteps ? chunk + 1u : chunk, s + 1u == kSteps ? 0u : s + 1u);
             if constexpr (i == NT - 1) xf[at].v = m + 1 < MT ? read_x(place, m + 1u, at) : read_x(next_place, 0u, at);
             if constexpr (m == MT - 1) {
                 f[i][at] = affine4_codes<XT>(word(raw[i], at));
@@ -636,13 +650,13 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
             if constexpr (kBehind) {
                 constexpr int kEach = 16 / kPer;
 #pragma unroll
-                for (int r = j * kEach; r < (j + 1) * kEach; ++r) into[r] = fmaf(before[0], old[r], into[r]);
+                for (int r = j * kEach; r < (j + 1) * kEach; ++r) into[r] = fmaf(chain ? factors[last / NT % kSubs][last % NT] : before, old[r], into[r]);
                 asm volatile("" : "+v"(into));
             }
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (!kBehind && j == kPer - 1) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[m][i][r] = fmaf(before[1], now[r], acc[m][i][r]);
+                for (int r = 0; r < 16; ++r) acc[m][i][r] = fmaf(factors[c][i], now[r], acc[m][i][r]);
                 asm volatile("" : "+v"(acc[m][i]));
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -669,7 +683,7 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
             const uint32_t skew = 8u * (meta_start(biases, 32u * i + col) & 2u);
             uint32_t words[kWords], pairs[4];
 #pragma unroll
-            for (uint32_t j = 0; j < kWords; ++j) words[j] = *reinterpret_cast<const uint32_t *>(run + j * 256u);
+            for (uint32_t j = 0; j < kWords; ++j) words[j] = *reinterpret_cast<const uint32_t *>(run + j * (128u * NT));
 #pragma unroll
             for (uint32_t j = 0; j + 1u < kWords; ++j) words[j] = __builtin_amdgcn_alignbit(words[j + 1u], words[j], skew);
 #pragma unroll
@@ -706,7 +720,7 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
 
     if (WM == 1 || wm == 0) load_metas(scales, L::kScales + wn * L::kMeta, 0);
     // as if steps -P ... -1 had asked for them
-    load_b(0, 0);
+    if (steps) load_b(0, 0);
 #pragma unroll
     for (int v = 0; v < P; ++v) {
         constexpr int kAhead = P % 2;  // v - P is odd where v is of the other parity than P
@@ -729,8 +743,9 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
         for (uint32_t j = 0; j < 4; ++j) xf[j].v = read_x(place, 0, j);
     };
     begin(0, 0, 0);
-    next_scale = scale_at(0, 0, 0);
+    read_scales(0, 0);
     uint32_t place = 0, unit = 0;
+    const uint32_t most_steps = min(chunks * kSteps, steps_in_all);
     for (uint32_t chunk = 0; chunk < chunks; ++chunk) {
         auto one = [&](uint32_t s, auto odd_) {
             const uint32_t g = chunk * kSteps + s, next_place = place == P - 1u ? 0u : place + 1u;
@@ -740,22 +755,48 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
             unit = next_unit;
         };
 #pragma unroll 1
-        for (uint32_t s = 0; s < kSteps && chunk * kSteps + s < steps; s += 2u) {
-            one(s, std::integral_constant<uint32_t, 0>{});
-            if (chunk * kSteps + s + 1u < steps) one(s + 1u, std::integral_constant<uint32_t, 1>{});
+        for (uint32_t s = 0; s < kSteps; s += 2u) {
+            const uint32_t g = chunk * kSteps + s;
+            if (KS == 1 && g >= steps) break;
+            // (a part that ends earlier meets the others all the same, as far as the first part, the longest, goes)
+            if (g < steps) one(s, std::integral_constant<uint32_t, 0>{});
+            else if (g < most_steps) wait_loads_and_sync<0>();
+            if (g + 1u < steps) one(s + 1u, std::integral_constant<uint32_t, 1>{});
+            else if (g + 1u < most_steps) wait_loads_and_sync<0>();
         }
         // the chunk's bias term, once every wave has formed its sums
-        const uint32_t chains = min(8u, SUB32 ? groups - chunk * 8u : steps - chunk * kSteps);
+        const uint32_t done = min(chunk * kSteps, steps), chains = min(8u, SUB32 ? my_groups - min(chunk * 8u, my_groups) : steps - done);
         if (chains < 8u) clear_sums(chains);
-        if (chunk + 1u == chunks) wait_loads_and_sync<0>();
-        else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        add_bias(chains);
+        if (done + kSteps >= steps) wait_loads<0>();  // (in the last one its biases may still be on their way)
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (chains) add_bias(chains);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         begin(place, unit, (chunk + 1u) * kSteps);  // (held across the bias term, the operands are spilled)
     }
 #pragma unroll
-    for (int r = 0; kBehind && r < 16; ++r) acc[MT - 1][NT - 1][r] = fmaf(before[1], p[kBehind][r], acc[MT - 1][NT - 1][r]);
+    for (int r = 0; kBehind && r < 16; ++r) acc[MT - 1][NT - 1][r] = fmaf(factors[kSubs - 1][NT - 1], p[kBehind][r], acc[MT - 1][NT - 1][r]);
     __syncthreads();
+    if constexpr (KS > 1) {  // the second part's sums by way of LDS; the first has the rest
+        static_assert(KS == 2);
+        float *const meet_at = reinterpret_cast<float *>(lds_of_parts) + wave * (MT * NT * 1024u) + lane;
+        if (part == 1u)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) meet_at[((m * NT + i) * 16 + r) * 64] = acc[m][i][r];
+        __syncthreads();
+        if (part == 0)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[m][i][r] = __fadd_rn(acc[m][i][r], meet_at[((m * NT + i) * 16 + r) * 64]);
+        __syncthreads();
+        if (part == 1u) return;
+    }
     if (!active) return;
 
     // ---- out: a block of 32 rows at a time through the wave's own part of LDS, so that a row's outputs leave 16 bytes a lane
@@ -797,11 +838,11 @@ __global__ __launch_bounds__(64 * WM * WN, NT == 4 ? 1 : 2) void k_affine4_tile(
     }
 }
 
-template <int XT, int GROUP, int MT, int NT, int WM, int WN, int P>
+template <int XT, int GROUP, int MT, int NT, int WM, int WN, int P, int KS>
 static int launch_tile(const Affine4Args &a, hipStream_t s) {
-    typedef TileLds<MT, NT, WM, WN, P> L;
-    hipLaunchKernelGGL((k_affine4_tile<XT, GROUP, MT, NT, WM, WN, P>), dim3((a.n + L::kOuts - 1u) / L::kOuts, (a.rows + L::kRows - 1u) / L::kRows),
-                       dim3(64u * L::kWaves), L::kBytes, s, a);
+    typedef TileLds<MT, NT, WM, WN, P, KS> L;
+    hipLaunchKernelGGL((k_affine4_tile<XT, GROUP, MT, NT, WM, WN, P, KS>), dim3((a.n + L::kOuts - 1u) / L::kOuts, (a.rows + L::kRows - 1u) / L::kRows),
+                       dim3(64u * L::kWaves * KS), KS * L::kBytes, s, a);
     SHRIKE_HIP(hipGetLastError());
     return 0;
 }
@@ -810,9 +851,9 @@ template <int XT, int GROUP>
 static int launch_affine4(const Affine4Args &a, hipStream_t s) {
     if (a.rows <= 8u) return launch_few<XT, GROUP, 1>(a, s);
     if (a.rows > 64u && a.x_stride * 512u < uint64_t(1) << 32) {  // (a tile's rows are reached by 32 bits)
-        if (uint64_t((a.n + 255u) / 256u) * ((a.rows + 255u) / 256u) >= 200u) return launch_tile<XT, GROUP, 4, 2, 2, 4, 3>(a, s);
-        if (uint64_t((a.n + 127u) / 128u) * ((a.rows + 127u) / 128u) >= 512u) return launch_tile<XT, GROUP, 4, 1, 1, 4, 3>(a, s);
-        return launch_tile<XT, GROUP, 2, 1, 1, 4, 4>(a, s);
+        if (uint64_t((a.n + 255u) / 256u) * ((a.rows + 255u) / 256u) >= 200u) return launch_tile<XT, GROUP, 4, 2, 2, 4, 3, 1>(a, s);
+        if (uint64_t((a.n + 127u) / 128u) * ((a.rows + 127u) / 128u) >= 200u) return launch_tile<XT, GROUP, 4, 1, 1, 4, 3, 2>(a, s);
+        return launch_tile<XT, GROUP, 2, 1, 1, 4, 4, 2>(a, s);
     }
     const uint64_t blocks = (a.n + 31u) / 32u;
     if (a.rows <= 16u || blocks * ((a.rows + 31u) / 32u) < 512u) return launch_few<XT, GROUP, 2>(a, s);
