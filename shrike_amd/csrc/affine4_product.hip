@@ -101,6 +101,171 @@ __device__ __forceinline__ void affine4_store(const Affine4Args &a, uint32_t r, 
     else static_cast<uint16_t *>(a.out)[at] = uint16_t(bf16_pair(v, 0.0f));
 }
 
+// ------------------------------------------------------------------ one row
+//
+// A matrix-vector product is the reading of its weights. Lanes side by side read a row's 16-byte chunks (32 codes) side by side: 2^shift lanes a
+// row, NCH chunks each, so that rows of any length leave few lanes idle (90 chunks of 2,880 k are three steps of 32 lanes, 94 %). A wave holds its
+// slices of x in registers and takes a batch of rows a turn, turn after turn. (A row of x too long for that is read piece by piece with every turn.)
+constexpr int kGemvChunks = 6;
+template <int NCH>
+constexpr int kGemvBatch = NCH <= 2 ? 4 : 2;  // rows a lane and turn: eight to twelve loads on their way
+
+struct GemvSlice {
+    uint32_t p[16];  // 32 values as pairs, in the order that the codes come in
+    float sum;
+};
+// fp16: pairs (0, 4) (1, 5) (2, 6) (3, 7) of eight; bf16: in order
+template <int XT>
+__device__ __forceinline__ void gemv_slice(GemvSlice &x, const uint4 (&v)[4]) {
+    x.sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (XT == SHRIKE_ELEM_F16) {
+            h2_t p[4];
+            pairs_from_x8(v[j], p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.p[4 * j + i] = as_u32(p[i]);
+        } else {
+            x.p[4 * j] = v[j].x;
+            x.p[4 * j + 1] = v[j].y;
+            x.p[4 * j + 2] = v[j].z;
+            x.p[4 * j + 3] = v[j].w;
+        }
+        x.sum = affine4_add<XT>(v[j], x.sum);
+    }
+}
+template <int XT>
+__device__ __forceinline__ float gemv_dot(const uint4 &w, const GemvSlice &x) {
+    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+    if constexpr (XT == SHRIKE_ELEM_F16) {
+        // a code in the low bits of 1024, or four bits further up in 64, is that number and the code; less the number it is the code, as a normal
+        // fp16 (of the subnormals that need no subtraction this instruction, too, drops what lies low: 4e-6 of the result of 2,880 k for 1e-7)
+        const h2_t k1024 = {_Float16(1024.0f), _Float16(1024.0f)}, k64 = {_Float16(64.0f), _Float16(64.0f)};
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t lo = words[j], hi = words[j] >> 8;
+            sum = __builtin_amdgcn_fdot2(as_h2((lo & 0x000f000fu) | 0x64006400u) - k1024, as_h2(x.p[4 * j]), sum, false);
+            sum = __builtin_amdgcn_fdot2(as_h2((lo & 0x00f000f0u) | 0x54005400u) - k64, as_h2(x.p[4 * j + 1]), sum, false);
+            sum = __builtin_amdgcn_fdot2(as_h2((hi & 0x000f000fu) | 0x64006400u) - k1024, as_h2(x.p[4 * j + 2]), sum, false);
+            sum = __builtin_amdgcn_fdot2(as_h2((hi & 0x00f000f0u) | 0x54005400u) - k64, as_h2(x.p[4 * j + 3]), sum, false);
+        }
+        return sum;
+    } else {
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const Affine4Frag f = affine4_codes<XT>(words[j]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2_t, f.u[i]), __builtin_bit_cast(bf2_t, x.p[4 * j + i]), sum, false);
+        }
+        return sum;
+    }
+}
+
+template <int XT, int NCH, bool ONCE>
+__global__ __launch_bounds__(256) void k_affine4_gemv(Affine4Args a, uint32_t shift, uint32_t turns) {
+    const uint32_t lane = threadIdx.x & 63u, wave = blockIdx.x * 4u + wave_index(), waves = gridDim.x * 4u;
+    const uint32_t cpr = a.k / 32u, per_row = a.k / 2u, groups = a.k / a.group, lanes = 1u << shift, rows = 64u >> shift;
+    const uint32_t sub = lane >> shift, col = lane & (lanes - 1u), group_shift = a.group == 32u ? 0u : a.group == 64u ? 1u : 2u;
+    const uint32_t segments = (cpr + NCH * lanes - 1u) / (NCH * lanes);
+    GemvSlice x[NCH];
+    auto load_x = [&](uint32_t segment) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const uint32_t c = (segment * NCH + i) * lanes + col;
+            uint4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = reinterpret_cast<const uint4 *>(a.x)[min(c, cpr - 1u) * 4u + j];
+                if (c >= cpr) v[j] = zero4();  // past the row's end the lane counts for nothing
+            }
+            gemv_slice<XT>(x[i], v);
+        }
+    };
+    if (segments == 1u) load_x(0);
+    for (uint32_t turn = 0; turn < turns; ++turn) {
+        const uint32_t first = (turn * waves + wave) * kGemvBatch<NCH> * rows;
+        if (first >= a.n) return;
+        uint32_t n[kGemvBatch<NCH>];
+        float acc[kGemvBatch<NCH>];
+#pragma unroll
+        for (int r = 0; r < kGemvBatch<NCH>; ++r) {
+            n[r] = first + r * rows + sub;
+            acc[r] = 0.0f;
+        }
+        for (uint32_t segment = 0; segment < segments; ++segment) {
+            uint4 w[kGemvBatch<NCH>][NCH];
+            uint16_t s[kGemvBatch<NCH>][NCH], b[kGemvBatch<NCH>][NCH];
+#pragma unroll
+            for (int r = 0; r < kGemvBatch<NCH>; ++r) {
+                const uint32_t row = min(n[r], a.n - 1u);
+                const uint8_t *codes = a.codes + uint64_t(row) * per_row;
+                const uint16_t *scales = a.scales + uint64_t(row) * groups, *biases = (a.biases ? a.biases : a.scales) + uint64_t(row) * groups;
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    const uint32_t c = min((segment * NCH + i) * lanes + col, cpr - 1u), g = c >> group_shift;
+                    const u32x4_t *from = reinterpret_cast<const u32x4_t *>(codes) + c;
+                    const u32x4_t v = ONCE ? __builtin_nontemporal_load(from) : *from;
+                    w[r][i] = make_uint4(v.x, v.y, v.z, v.w);
+                    s[r][i] = scales[g];
+                    b[r][i] = biases[g];
+                }
+            }
+            if (segments > 1u) load_x(segment);
+#pragma unroll
+            for (int r = 0; r < kGemvBatch<NCH>; ++r)
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    const float scale = meta_f32(s[r][i], a.meta), bias = a.biases ? meta_f32(b[r][i], a.meta) : -8.0f * scale;
+                    acc[r] = fmaf(bias, x[i].sum, fmaf(scale, gemv_dot<XT>(w[r][i], x[i]), acc[r]));
+                }
+        }
+#pragma unroll
+        for (int r = 0; r < kGemvBatch<NCH>; ++r) acc[r] = seg_sum(acc[r], lanes);
+#pragma unroll
+        for (int r = 0; r < kGemvBatch<NCH>; ++r)
+            if (col == lanes - 1u && n[r] < a.n) affine4_store(a, 0, n[r], a.bias ? __fadd_rn(acc[r], meta_f32(a.bias[n[r]], a.meta)) : acc[r]);
+    }
+}
+
+template <int XT, int NCH>
+static int launch_gemv(const Affine4Args &a, uint32_t shift, hipStream_t s) {
+    // as many workgroups as the device holds at once; where there are more rows, each takes several turns, all of them as many
+    const uint64_t batches = (a.n + kGemvBatch<NCH> * (64u >> shift) - 1u) / (kGemvBatch<NCH> * (64u >> shift)), groups_of_waves = (batches + 3u) / 4u;
+    const uint32_t most = 256u * (NCH == 1 ? 5u : NCH <= 4 ? 3u : 2u), turns = uint32_t((groups_of_waves + most - 1u) / most);
+    const uint32_t workgroups = uint32_t((groups_of_waves + turns - 1u) / turns);
+    // weights that no cache holds are read with the hint that they will not be wanted again
+    if (uint64_t(a.n) * a.k / 2u >= uint64_t(192) << 20) hipLaunchKernelGGL((k_affine4_gemv<XT, NCH, true>), dim3(workgroups), dim3(256), 0, s, a, shift, turns);
+    else hipLaunchKernelGGL((k_affine4_gemv<XT, NCH, false>), dim3(workgroups), dim3(256), 0, s, a, shift, turns);
+    SHRIKE_HIP(hipGetLastError());
+    return 0;
+}
+template <int XT>
+static int launch_gemv(const Affine4Args &a, hipStream_t s) {
+    // the lanes a row: of those whose share fits, the one that leaves the fewest idle, and of equals the most
+    const uint32_t cpr = a.k / 32u;
+    uint32_t best = 6, steps = kGemvChunks, idle = ~0u;
+    for (uint32_t shift = 6; shift >= 2u; --shift) {
+        const uint32_t n = ((cpr - 1u) >> shift) + 1u;
+        if (n > uint32_t(kGemvChunks)) break;
+        const uint32_t left = ((n << shift) - cpr) * 256u / (n << shift);
+        if (left + 8u < idle) {  // (a gain of 3 % is worth its registers)
+            idle = left;
+            best = shift;
+            steps = n;
+        }
+    }
+    switch (steps) {
+    case 1: return launch_gemv<XT, 1>(a, best, s);
+    case 2: return launch_gemv<XT, 2>(a, best, s);
+    case 3: return launch_gemv<XT, 3>(a, best, s);
+    case 4: return launch_gemv<XT, 4>(a, best, s);
+    case 5: return launch_gemv<XT, 5>(a, best, s);
+    default: return launch_gemv<XT, 6>(a, best, s);
+    }
+}
+
 // Loads from where `at` bytes of a tensor of `bytes` lie, up to its end.
 typedef __amdgpu_buffer_rsrc_t buffer_t;
 __device__ __forceinline__ buffer_t affine4_buffer(const void *tensor, uint64_t at, uint64_t bytes) {
@@ -861,6 +1026,7 @@ static int launch_affine4(const Affine4Args &a, hipStream_t s) {
 }
 template <int XT>
 static int launch_affine4(const Affine4Args &a, hipStream_t s) {
+    if (a.rows == 1u) return launch_gemv<XT>(a, s);
     if (a.group == 32u) return launch_affine4<XT, 32>(a, s);
     return a.group == 64u ? launch_affine4<XT, 64>(a, s) : launch_affine4<XT, 128>(a, s);
 }
