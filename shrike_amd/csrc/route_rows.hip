@@ -17,6 +17,7 @@ struct RouteArgs {
     uint32_t rows, experts, top_k, groups, kept, group_size;
     uint32_t logits_type, bias_type, weights_type, group_top, sigmoid, renormalize;
     float scaling;
+    uint32_t whole;  // rows start at multiples of 16 bytes and are multiples of 16 bytes long
 };
 
 __device__ __forceinline__ float route_load(const void *p, uint64_t i, uint32_t type) {
@@ -175,6 +176,300 @@ __global__ __launch_bounds__(256) void k_route_rows(RouteArgs a) {
     for (uint64_t row = uint64_t(blockIdx.x) * 4u + wave; row < a.rows; row += uint64_t(gridDim.x) * 4u) route_row<NPL>(a, uint32_t(row), s_value[wave]);
 }
 
+// ------------------------------------------------------------------ many rows at once
+//
+// 64 bits are needed where two choices lie close together, and that is seldom: here a choice is a 32-bit word, its value in fixed point below the row's
+// largest (22 bits) over the expert's number (10, so that the lower one is the larger word), from fp32 arithmetic whose error is under two
+// units. The words' order is the choices' order where neighbours in it, the last one taken and the first one left among them, are kCertain units
+// apart; a row where they are not is routed again by route_row. (Of 16,384 rows of 512 experts with a bias 0.4 % are.) Where the logits
+// themselves decide and have 16 bits, the word is all of them over the number, and exact.
+//
+// LANES lanes have a row, each NPL neighbouring experts: 64 for few rows, which takes the fewest steps, 16 for many, where four rows share every step
+// between lanes. A step of the selection is the largest word of a lane's, of the row's lanes, and that one taken out.
+
+enum class RouteWord { kValue, kLogit, kLogit16 };
+constexpr uint32_t kCertain = 6;
+constexpr float kUnits = 4194296.0f;  // 2^22 - 8
+
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    if constexpr (LANES == 64) return wave_max_u32(v);
+    v = max(v, dpp_keep_u32<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = max(v, dpp_keep_u32<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = max(v, dpp_keep_u32<0x141>(v));  // row_half_mirror
+    return max(v, dpp_keep_u32<0x140>(v));  // row_mirror
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v) {
+    if constexpr (LANES == 64) return wave_max_f32(v);
+    v = fmaxf(v, dpp_keep_f32<0xB1>(v));
+    v = fmaxf(v, dpp_keep_f32<0x4E>(v));
+    v = fmaxf(v, dpp_keep_f32<0x141>(v));
+    return fmaxf(v, dpp_keep_f32<0x140>(v));
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+    if constexpr (LANES == 64) return wave_sum(v);
+    v += dpp_f32<0xB1>(v);
+    v += dpp_f32<0x4E>(v);
+    v += dpp_f32<0x141>(v);
+    return v + dpp_f32<0x140>(v);
+}
+__device__ __forceinline__ float exp_fast(float v) { return __builtin_amdgcn_exp2f(1.4426950408889634f * v); }
+
+template <int LANES, int NPL, RouteWord WORD>
+__global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
+    constexpr int kWide = LANES * NPL < 64 ? 1 : LANES * NPL / 64;  // experts a lane where a wave has the row
+    constexpr uint32_t kIndexBits = WORD == RouteWord::kLogit16 ? 16 : 10, kRows = 64 / LANES, kSlots = LANES == 16 ? 2 : 1;
+    constexpr uint32_t kOutWord = WORD == RouteWord::kLogit16 ? 0 : 1;  // what an expert out of service has above its number
+    __shared__ double s_value[4][64 * kWide];
+    const uint32_t lane = threadIdx.x & 63u, wave = wave_index(), sub = lane % LANES;
+    const uint64_t first_row = (uint64_t(blockIdx.x) * 4u + wave) * kRows;
+    if (first_row >= a.rows) return;
+    const bool real = first_row + lane / LANES < a.rows;
+    const uint64_t row = real ? first_row + lane / LANES : a.rows - 1u, at = row * a.stride;
+
+    // ---- the row
+    float l[NPL];
+    uint16_t bits[NPL];  // 16-bit logits as they are
+    if (a.logits_type == SHRIKE_ELEM_F32) {
+        const float *p = static_cast<const float *>(a.logits) + at + sub * NPL;
+        if (NPL % 4 == 0 && a.whole) {
+#pragma unroll
+            for (int j = 0; j < NPL; j += 4) {
+                const bool there = sub * NPL + j < a.experts;
+                const float4 v = *reinterpret_cast<const float4 *>(there ? p + j : static_cast<const float *>(a.logits) + at);
+                l[j] = v.x;
+                if (NPL > 1) l[j + 1 < NPL ? j + 1 : 0] = v.y, l[j + 2 < NPL ? j + 2 : 0] = v.z, l[j + 3 < NPL ? j + 3 : 0] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) l[j] = static_cast<const float *>(a.logits)[at + min(sub * NPL + j, a.experts - 1u)];
+        }
+    } else {
+        const uint16_t *p = static_cast<const uint16_t *>(a.logits) + at;
+        if (NPL % 8 == 0 && a.whole) {
+#pragma unroll
+            for (int j = 0; j < NPL; j += 8) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(p + (sub * NPL + j < a.experts ? sub * NPL + j : 0u));
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) bits[(j + i) % NPL] = uint16_t(w[i / 2] >> 16 * (i % 2));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) bits[j] = p[min(sub * NPL + j, a.experts - 1u)];
+        }
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) l[j] = a.logits_type == SHRIKE_ELEM_F16 ? f16_to_f32(bits[j]) : bf16_to_f32(bits[j]);
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) {
+        l[j] = sub * NPL + j < a.experts ? in_service(l[j]) : -INFINITY;
+        top = fmaxf(top, l[j]);
+    }
+    top = lanes_max<LANES>(top);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float inverse = 0.0f;  // of the softmax's sum, where it is wanted
+    if (!a.sigmoid && (WORD == RouteWord::kValue || !a.renormalize)) {
+        float total = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) total += exp_fast(l[j] - base);
+        total = lanes_sum<LANES>(total);
+        inverse = total > 0.0f ? __builtin_amdgcn_rcpf(total) : 0.0f;
+    }
+    auto score = [&](float v) { return a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_fast(-v)) : exp_fast(v - base) * inverse; };
+
+    // ---- the words
+    uint32_t key[NPL];
+    bool certain = true;
+    if constexpr (WORD == RouteWord::kLogit16) {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) {
+            const uint32_t e = sub * NPL + j, b = bits[j] == 0x8000u ? 0u : bits[j], order = (b & 0x8000u ? ~b : b | 0x8000u) & 0xffffu;
+            key[j] = e >= a.experts ? 0u : (l[j] == -INFINITY ? 0u : order << 16) | (1024u - e);
+        }
+    } else {
+        float v[NPL], most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) {
+            v[j] = l[j];
+            if constexpr (WORD == RouteWord::kValue) {
+                v[j] = l[j] == -INFINITY ? -INFINITY : score(l[j]);
+                if (a.bias) v[j] += in_service(route_load(a.bias, min(sub * NPL + j, a.experts - 1u), a.bias_type));
+            }
+            most = fmaxf(most, v[j]);
+        }
+        most = lanes_max<LANES>(most);
+        constexpr float kSpan = WORD == RouteWord::kValue ? 2.0f : 32.0f;
+        if (WORD == RouteWord::kValue) certain = most == -INFINITY || fabsf(most) <= 4.0f;  // (further off, an fp32 is too coarse)
+        const float low = most - kSpan;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) {
+            const uint32_t e = sub * NPL + j;
+            // 2: as far below the largest as the word reaches, or further
+            const uint32_t q = v[j] == -INFINITY ? kOutWord : min(max(uint32_t(fmaxf((v[j] - low) * (kUnits / kSpan), 0.0f)), 2u), 0x3fffffu);
+            key[j] = e >= a.experts ? 0u : q << 10 | (1023u - e);
+        }
+    }
+    // a ahead of b for certain, by the parts above their numbers
+    auto ahead = [&](uint32_t a_, uint32_t b_, uint32_t apart) { return WORD == RouteWord::kLogit16 || b_ <= kOutWord || a_ >= b_ + apart; };
+
+    // ---- groups: whole lanes, 2^i of them, have one
+    if (a.groups > 1u) {
+        const uint32_t lanes = a.group_size / NPL, group = sub / lanes;
+        uint32_t best = 0, second = 0;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) {
+            const uint32_t q = key[j] >> kIndexBits;
+            second = max(second, min(best, q));
+            best = max(best, q);
+        }
+        auto merge = [&](uint32_t o1, uint32_t o2) {
+            second = max(max(second, o2), min(best, o1));
+            best = max(best, o1);
+        };
+        if (lanes >= 2u) merge(dpp_keep_u32<0xB1>(best), dpp_keep_u32<0xB1>(second));
+        if (lanes >= 4u) merge(dpp_keep_u32<0x4E>(best), dpp_keep_u32<0x4E>(second));
+        if (lanes >= 8u) merge(dpp_keep_u32<0x141>(best), dpp_keep_u32<0x141>(second));
+        if (lanes >= 16u) merge(dpp_keep_u32<0x140>(best), dpp_keep_u32<0x140>(second));
+        uint32_t mark = best, apart = kCertain;
+        bool known = true;
+        if (WORD != RouteWord::kLogit16 && a.group_top == 2u && best > kOutWord) {
+            known = second > 2u && best > 2u;  // (what is missing counts 0, and what lies too low is not known: both by route_row)
+            mark = best + second;
+            apart = 2u * kCertain;
+        }
+        if (WORD != RouteWord::kLogit16) known &= best != 2u;
+        const bool counts = sub * NPL < a.experts;
+        uint32_t word = counts ? (mark + 1u) << 6 | (63u - group) : 0u, last = 0;
+        bool kept = false;
+        for (uint32_t r = 0; r < a.kept; ++r) {
+            last = lanes_max<LANES>(word);
+            const bool mine = word == last;
+            kept |= mine;
+            word = mine ? 0u : word;
+        }
+        const uint32_t left = lanes_max<LANES>(word);
+        certain &= ahead((last >> 6) - 1u, (left >> 6) - 1u, apart);
+        certain &= lanes_max<LANES>(counts && !known ? 1u : 0u) == 0u;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) key[j] = kept ? key[j] : 0u;
+    }
+
+    // ---- the top k
+    uint32_t won[kSlots] = {};  // of rank sub, and sub + 16
+    uint32_t before = 0;
+    auto largest = [&] {
+        uint32_t best = key[0];
+#pragma unroll
+        for (int j = 1; j < NPL; ++j) best = max(best, key[j]);
+        return lanes_max<LANES>(best);
+    };
+    for (uint32_t r = 0; r < a.top_k; ++r) {
+        const uint32_t most = largest();
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) key[j] = key[j] == most ? 0u : key[j];
+        if (r) certain &= ahead(before >> kIndexBits, most >> kIndexBits, kCertain);
+        before = most;
+#pragma unroll
+        for (uint32_t i = 0; i < kSlots; ++i) won[i] = sub + i * LANES == r ? most : won[i];
+    }
+    if (WORD != RouteWord::kLogit16) {
+        const uint32_t left = largest();
+        certain &= left == 0u || ahead(before >> kIndexBits, left >> kIndexBits, kCertain);
+    }
+
+    // ---- the weights
+    uint32_t index[kSlots];
+    float w[kSlots], most = -INFINITY, sum = 0.0f;
+    bool served[kSlots];
+#pragma unroll
+    for (uint32_t i = 0; i < kSlots; ++i) {
+        const bool on = sub + i * LANES < a.top_k;
+        index[i] = on ? (WORD == RouteWord::kLogit16 ? 1024u - (won[i] & 0xffffu) : 1023u - (won[i] & 0x3ffu)) : 0u;
+        served[i] = on && (won[i] >> kIndexBits) > kOutWord;
+        w[i] = in_service(route_load(a.logits, at + min(index[i], a.experts - 1u), a.logits_type));
+        most = fmaxf(most, served[i] ? w[i] : -INFINITY);
+    }
+    const bool among = a.renormalize && !a.sigmoid;  // the softmax of the chosen ones
+    most = among ? lanes_max<LANES>(most) : 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < kSlots; ++i) {
+        w[i] = !served[i] ? 0.0f : among ? exp_fast(w[i] - most) : score(w[i]);
+        sum += w[i];
+    }
+    if (a.renormalize) {
+        sum = lanes_sum<LANES>(sum);
+        // (scores that fp32 does not hold well are 64 bits' again; none in service leaves zeros)
+        if (a.sigmoid) certain &= sum > 1e-30f || lanes_max<LANES>(served[0] ? 1u : 0u) == 0u;
+        const float factor = sum > 0.0f ? a.scaling / sum : 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < kSlots; ++i) w[i] *= factor;
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kSlots; ++i) w[i] *= a.scaling;
+    }
+    if (real && certain)
+#pragma unroll
+        for (uint32_t i = 0; i < kSlots; ++i)
+            if (sub + i * LANES < a.top_k) {
+                a.indices[row * a.top_k + sub + i * LANES] = index[i];
+                route_store_weight(a, row * a.top_k + sub + i * LANES, double(w[i]));
+            }
+    // ---- rows that are not certain, one by one by the whole wave
+    for (uint64_t again = __ballot(real && !certain && sub == 0); again; again &= again - 1u)
+        route_row<kWide>(a, uint32_t(first_row + __builtin_ctzll(again) / LANES), s_value[wave]);
+}
+
+template <int LANES, int NPL>
+static void launch_route_fast(const RouteArgs &a, hipStream_t s) {
+    const uint32_t per = 4u * (64u / LANES), blocks = uint32_t((uint64_t(a.rows) + per - 1u) / per);
+    const bool by_value = a.bias || (a.groups > 1u && a.group_top == 2u);
+    if (by_value) hipLaunchKernelGGL((k_route_rows_fast<LANES, NPL, RouteWord::kValue>), dim3(blocks), dim3(256), 0, s, a);
+    else if (a.logits_type == SHRIKE_ELEM_F32) hipLaunchKernelGGL((k_route_rows_fast<LANES, NPL, RouteWord::kLogit>), dim3(blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_route_rows_fast<LANES, NPL, RouteWord::kLogit16>), dim3(blocks), dim3(256), 0, s, a);
+}
+// the experts a lane for a row of 2^i lanes
+static uint32_t experts_a_lane(uint32_t experts, uint32_t lanes) {
+    uint32_t n = 1;
+    while (n * lanes < experts) n *= 2u;
+    return n;
+}
+constexpr uint32_t kRowsForNarrow = 2048;
+// Whether groups are 2^i whole lanes, up to 16.
+static bool groups_are_lanes(const RouteArgs &a, uint32_t per_lane) {
+    if (a.groups == 1u) return true;
+    const uint32_t lanes = a.group_size / per_lane;
+    return a.group_size % per_lane == 0 && lanes <= 16u && (lanes & (lanes - 1u)) == 0;
+}
+
+static void launch_route(const RouteArgs &a, hipStream_t s) {
+    const uint32_t wide = experts_a_lane(a.experts, 64), narrow = experts_a_lane(a.experts, 16);
+    if (a.rows >= kRowsForNarrow && narrow <= 32u && groups_are_lanes(a, narrow)) {
+        if (narrow <= 1u) launch_route_fast<16, 1>(a, s);
+        else if (narrow == 2u) launch_route_fast<16, 2>(a, s);
+        else if (narrow == 4u) launch_route_fast<16, 4>(a, s);
+        else if (narrow == 8u) launch_route_fast<16, 8>(a, s);
+        else if (narrow == 16u) launch_route_fast<16, 16>(a, s);
+        else launch_route_fast<16, 32>(a, s);
+    } else if (groups_are_lanes(a, wide)) {
+        if (wide <= 1u) launch_route_fast<64, 1>(a, s);
+        else if (wide == 2u) launch_route_fast<64, 2>(a, s);
+        else if (wide == 4u) launch_route_fast<64, 4>(a, s);
+        else if (wide == 8u) launch_route_fast<64, 8>(a, s);
+        else launch_route_fast<64, 16>(a, s);
+    } else {
+        const dim3 blocks(std::min((a.rows - 1u) / 4u + 1u, 65536u)), threads(256);
+        if (wide <= 1u) hipLaunchKernelGGL((k_route_rows<1>), blocks, threads, 0, s, a);
+        else if (wide == 2u) hipLaunchKernelGGL((k_route_rows<2>), blocks, threads, 0, s, a);
+        else if (wide == 4u) hipLaunchKernelGGL((k_route_rows<4>), blocks, threads, 0, s, a);
+        else if (wide == 8u) hipLaunchKernelGGL((k_route_rows<8>), blocks, threads, 0, s, a);
+        else hipLaunchKernelGGL((k_route_rows<16>), blocks, threads, 0, s, a);
+    }
+}
+
 }  // namespace shrike
 
 using namespace shrike;
@@ -223,14 +518,18 @@ extern "C" int shrike_hip_route_rows(void *stream, const shrike_route_desc *desc
     a.sigmoid = desc->scores == SHRIKE_SCORES_SIGMOID;
     a.renormalize = desc->renormalize != 0;
     a.scaling = desc->scaling;
-    const uint32_t blocks = std::min((rows - 1u) / 4u + 1u, 65536u);
-    const hipStream_t s = as_stream(stream);
-    const uint32_t per_lane = (a.experts + 63u) / 64u;
-    if (per_lane <= 1) hipLaunchKernelGGL((k_route_rows<1>), dim3(blocks), dim3(256), 0, s, a);
-    else if (per_lane <= 2) hipLaunchKernelGGL((k_route_rows<2>), dim3(blocks), dim3(256), 0, s, a);
-    else if (per_lane <= 4) hipLaunchKernelGGL((k_route_rows<4>), dim3(blocks), dim3(256), 0, s, a);
-    else if (per_lane <= 8) hipLaunchKernelGGL((k_route_rows<8>), dim3(blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_route_rows<16>), dim3(blocks), dim3(256), 0, s, a);
-    SHRIKE_HIP(hipGetLastError());
+    const uint64_t size_of = logits_dtype == SHRIKE_ELEM_F32 ? 4u : 2u;
+    a.whole = reinterpret_cast<uintptr_t>(d_logits) % 16u == 0 && (rows == 1u || logits_stride_elements * size_of % 16u == 0) && a.experts * size_of % 16u == 0;
+    constexpr uint32_t kMostRows = 1u << 24;  // of a launch, which holds fewer than 2^32 threads
+    for (uint32_t done = 0; done < rows; done += kMostRows) {
+        RouteArgs part = a;
+        part.rows = std::min(rows - done, kMostRows);
+        part.logits = static_cast<const uint8_t *>(d_logits) + uint64_t(done) * logits_stride_elements * size_of;
+        part.indices = d_out_indices + uint64_t(done) * a.top_k;
+        part.weights = static_cast<uint8_t *>(d_out_weights) + uint64_t(done) * a.top_k * (weights_dtype == SHRIKE_ELEM_F32 ? 4u : 2u);
+        launch_route(part, as_stream(stream));
+        SHRIKE_HIP(hipGetLastError());
+        if (rows - done <= kMostRows) break;
+    }
     return 0;
 }
