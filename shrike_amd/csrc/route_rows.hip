@@ -17,7 +17,7 @@ struct RouteArgs {
     uint32_t rows, experts, top_k, groups, kept, group_size;
     uint32_t logits_type, bias_type, weights_type, group_top, sigmoid, renormalize;
     float scaling;
-    uint32_t whole;  // rows start at multiples of 16 bytes and are multiples of 16 bytes long
+    uint32_t whole, whole_bias;  // rows (the bias) start at multiples of 16 bytes and are multiples of 16 bytes long
 };
 
 __device__ __forceinline__ float route_load(const void *p, uint64_t i, uint32_t type) {
@@ -180,15 +180,14 @@ __global__ __launch_bounds__(256) void k_route_rows(RouteArgs a) {
 //
 // 64 bits are needed where two choices lie close together, and that is seldom: here a choice is a 32-bit word, its value in fixed point below the row's
 // largest (22 bits) over the expert's number (10, so that the lower one is the larger word), from fp32 arithmetic whose error is under two
-// units. The words' order is the choices' order where neighbours in it, the last one taken and the first one left among them, are kCertain units
-// apart; a row where they are not is routed again by route_row. (Of 16,384 rows of 512 experts with a bias 0.4 % are.) Where the logits
+// units. The words' order is the choices' order where neighbours in it, the last one taken and the first one left among them, are as far
+// apart as both may be off; a row where they are not is routed again by route_row. Where the logits
 // themselves decide and have 16 bits, the word is all of them over the number, and exact.
 //
 // LANES lanes have a row, each NPL neighbouring experts: 64 for few rows, which takes the fewest steps, 16 for many, where four rows share every step
-// between lanes. A step of the selection is the largest word of a lane's, of the row's lanes, and that one taken out.
+// between lanes. A step of the selection is the largest of a lane's words below the last one taken, and then of the row's lanes.
 
 enum class RouteWord { kValue, kLogit, kLogit16 };
-constexpr uint32_t kCertain = 6;
 constexpr float kUnits = 4194296.0f;  // 2^22 - 8
 
 template <int LANES>
@@ -217,6 +216,49 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 __device__ __forceinline__ float exp_fast(float v) { return __builtin_amdgcn_exp2f(1.4426950408889634f * v); }
 
+// NPL neighbouring values from `at` on for the sub-th lane of a row, and their 16 bits where they have 16; past the last expert something. `whole`: from 16-byte
+// aligned addresses, in whole loads.
+template <int NPL>
+__device__ __forceinline__ void load_experts(const void *from, uint64_t at, uint32_t type, uint32_t whole, uint32_t sub, uint32_t experts, float (&v)[NPL],
+                                             uint16_t (&bits)[NPL]) {
+    if (type == SHRIKE_ELEM_F32) {
+        const float *p = static_cast<const float *>(from) + at;
+        if (NPL % 4 == 0 && whole) {
+#pragma unroll
+            for (int j = 0; j < NPL; j += 4) {
+                const float4 f = *reinterpret_cast<const float4 *>(p + (sub * NPL + j < experts ? sub * NPL + j : 0u));
+                const float w[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[(j + i) % NPL] = w[i];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) v[j] = p[min(sub * NPL + j, experts - 1u)];
+        }
+        return;
+    }
+    const uint16_t *p = static_cast<const uint16_t *>(from) + at;
+    if (NPL % 8 == 0 && whole) {
+#pragma unroll
+        for (int j = 0; j < NPL; j += 8) {
+            const uint4 f = *reinterpret_cast<const uint4 *>(p + (sub * NPL + j < experts ? sub * NPL + j : 0u));
+            const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bits[(j + i) % NPL] = uint16_t(w[i / 2] >> 16 * (i % 2));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) bits[j] = p[min(sub * NPL + j, experts - 1u)];
+    }
+    if (type == SHRIKE_ELEM_F16) {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) v[j] = f16_to_f32(bits[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) v[j] = bf16_to_f32(bits[j]);
+    }
+}
+
 template <int LANES, int NPL, RouteWord WORD>
 __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     constexpr int kWide = LANES * NPL < 64 ? 1 : LANES * NPL / 64;  // experts a lane where a wave has the row
@@ -230,38 +272,14 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     const uint64_t row = real ? first_row + lane / LANES : a.rows - 1u, at = row * a.stride;
 
     // ---- the row
-    float l[NPL];
+    float l[NPL], b[NPL];
     uint16_t bits[NPL];  // 16-bit logits as they are
-    if (a.logits_type == SHRIKE_ELEM_F32) {
-        const float *p = static_cast<const float *>(a.logits) + at + sub * NPL;
-        if (NPL % 4 == 0 && a.whole) {
+    load_experts<NPL>(a.logits, at, a.logits_type, a.whole, sub, a.experts, l, bits);
+    if (WORD == RouteWord::kValue) {
 #pragma unroll
-            for (int j = 0; j < NPL; j += 4) {
-                const bool there = sub * NPL + j < a.experts;
-                const float4 v = *reinterpret_cast<const float4 *>(there ? p + j : static_cast<const float *>(a.logits) + at);
-                l[j] = v.x;
-                if (NPL > 1) l[j + 1 < NPL ? j + 1 : 0] = v.y, l[j + 2 < NPL ? j + 2 : 0] = v.z, l[j + 3 < NPL ? j + 3 : 0] = v.w;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < NPL; ++j) l[j] = static_cast<const float *>(a.logits)[at + min(sub * NPL + j, a.experts - 1u)];
-        }
-    } else {
-        const uint16_t *p = static_cast<const uint16_t *>(a.logits) + at;
-        if (NPL % 8 == 0 && a.whole) {
-#pragma unroll
-            for (int j = 0; j < NPL; j += 8) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(p + (sub * NPL + j < a.experts ? sub * NPL + j : 0u));
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) bits[(j + i) % NPL] = uint16_t(w[i / 2] >> 16 * (i % 2));
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < NPL; ++j) bits[j] = p[min(sub * NPL + j, a.experts - 1u)];
-        }
-#pragma unroll
-        for (int j = 0; j < NPL; ++j) l[j] = a.logits_type == SHRIKE_ELEM_F16 ? f16_to_f32(bits[j]) : bf16_to_f32(bits[j]);
+        for (int j = 0; j < NPL; ++j) b[j] = 0.0f;
+        uint16_t unused[NPL];
+        if (a.bias) load_experts<NPL>(a.bias, 0, a.bias_type, a.whole_bias, sub, a.experts, b, unused);
     }
     float top = -INFINITY;
 #pragma unroll
@@ -282,39 +300,47 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     auto score = [&](float v) { return a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_fast(-v)) : exp_fast(v - base) * inverse; };
 
     // ---- the words
-    uint32_t key[NPL];
+    uint32_t key[NPL], apart = 3;  // units that two choices have to be apart
     bool certain = true;
     if constexpr (WORD == RouteWord::kLogit16) {
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
-            const uint32_t e = sub * NPL + j, b = bits[j] == 0x8000u ? 0u : bits[j], order = (b & 0x8000u ? ~b : b | 0x8000u) & 0xffffu;
+            const uint32_t e = sub * NPL + j, as_is = bits[j] == 0x8000u ? 0u : bits[j], order = (as_is & 0x8000u ? ~as_is : as_is | 0x8000u) & 0xffffu;
             key[j] = e >= a.experts ? 0u : (l[j] == -INFINITY ? 0u : order << 16) | (1024u - e);
         }
     } else {
-        float v[NPL], most = -INFINITY;
+        float v[NPL], most = -INFINITY, least = INFINITY;
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
             v[j] = l[j];
             if constexpr (WORD == RouteWord::kValue) {
-                v[j] = l[j] == -INFINITY ? -INFINITY : score(l[j]);
-                if (a.bias) v[j] += in_service(route_load(a.bias, min(sub * NPL + j, a.experts - 1u), a.bias_type));
+                float value = score(l[j]) + in_service(b[j]);
+                asm volatile("" : "+v"(value));  // (or the compiler branches round it, lane by lane)
+                v[j] = l[j] == -INFINITY ? -INFINITY : value;
             }
             most = fmaxf(most, v[j]);
+            if (WORD == RouteWord::kValue) least = fminf(least, v[j] == -INFINITY ? INFINITY : v[j]);
         }
         most = lanes_max<LANES>(most);
-        constexpr float kSpan = WORD == RouteWord::kValue ? 2.0f : 32.0f;
-        if (WORD == RouteWord::kValue) certain = most == -INFINITY || fabsf(most) <= 4.0f;  // (further off, an fp32 is too coarse)
-        const float low = most - kSpan;
+        float span = 32.0f;
+        if constexpr (WORD == RouteWord::kValue) {
+            // all the row's choices, or as far down as 2; a choice is off by the score's few last places and by half a one of its own
+            span = fminf(fmaxf(most + lanes_max<LANES>(-least), 0x1p-10f), 2.0f);
+            certain = most == -INFINITY || fabsf(most) <= 4.0f;  // (further off, an fp32 is too coarse)
+            const float off = (a.sigmoid ? 1.0f : inverse) * 0x1p-22f + (fabsf(most) + span) * 0x1p-24f;
+            apart = 3u + uint32_t(2.0f * off * (kUnits / span));
+        }
+        const float low = most - span, per_unit = kUnits / span;
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
             const uint32_t e = sub * NPL + j;
             // 2: as far below the largest as the word reaches, or further
-            const uint32_t q = v[j] == -INFINITY ? kOutWord : min(max(uint32_t(fmaxf((v[j] - low) * (kUnits / kSpan), 0.0f)), 2u), 0x3fffffu);
+            const uint32_t q = v[j] == -INFINITY ? kOutWord : min(max(uint32_t(fmaxf((v[j] - low) * per_unit, 0.0f)), 2u), 0x3fffffu);
             key[j] = e >= a.experts ? 0u : q << 10 | (1023u - e);
         }
     }
     // a ahead of b for certain, by the parts above their numbers
-    auto ahead = [&](uint32_t a_, uint32_t b_, uint32_t apart) { return WORD == RouteWord::kLogit16 || b_ <= kOutWord || a_ >= b_ + apart; };
+    auto ahead = [&](uint32_t a_, uint32_t b_, uint32_t by) { return WORD == RouteWord::kLogit16 || b_ <= kOutWord || a_ >= b_ + by; };
 
     // ---- groups: whole lanes, 2^i of them, have one
     if (a.groups > 1u) {
@@ -334,12 +360,12 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
         if (lanes >= 4u) merge(dpp_keep_u32<0x4E>(best), dpp_keep_u32<0x4E>(second));
         if (lanes >= 8u) merge(dpp_keep_u32<0x141>(best), dpp_keep_u32<0x141>(second));
         if (lanes >= 16u) merge(dpp_keep_u32<0x140>(best), dpp_keep_u32<0x140>(second));
-        uint32_t mark = best, apart = kCertain;
+        uint32_t mark = best, by = apart;
         bool known = true;
         if (WORD != RouteWord::kLogit16 && a.group_top == 2u && best > kOutWord) {
             known = second > 2u && best > 2u;  // (what is missing counts 0, and what lies too low is not known: both by route_row)
             mark = best + second;
-            apart = 2u * kCertain;
+            by = 2u * apart;
         }
         if (WORD != RouteWord::kLogit16) known &= best != 2u;
         const bool counts = sub * NPL < a.experts;
@@ -352,7 +378,7 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
             word = mine ? 0u : word;
         }
         const uint32_t left = lanes_max<LANES>(word);
-        certain &= ahead((last >> 6) - 1u, (left >> 6) - 1u, apart);
+        certain &= ahead((last >> 6) - 1u, (left >> 6) - 1u, by);
         certain &= lanes_max<LANES>(counts && !known ? 1u : 0u) == 0u;
 #pragma unroll
         for (int j = 0; j < NPL; ++j) key[j] = kept ? key[j] : 0u;
@@ -361,24 +387,23 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     // ---- the top k
     uint32_t won[kSlots] = {};  // of rank sub, and sub + 16
     uint32_t before = 0;
-    auto largest = [&] {
-        uint32_t best = key[0];
+    // the largest word below `taken` (0: of all): less `taken`, what lies below it wraps round above what does not, in its order
+    auto largest_below = [&](uint32_t taken) {
+        uint32_t best = key[0] - taken;
 #pragma unroll
-        for (int j = 1; j < NPL; ++j) best = max(best, key[j]);
-        return lanes_max<LANES>(best);
+        for (int j = 1; j < NPL; ++j) best = max(best, key[j] - taken);
+        return lanes_max<LANES>(best) + taken;
     };
     for (uint32_t r = 0; r < a.top_k; ++r) {
-        const uint32_t most = largest();
-#pragma unroll
-        for (int j = 0; j < NPL; ++j) key[j] = key[j] == most ? 0u : key[j];
-        if (r) certain &= ahead(before >> kIndexBits, most >> kIndexBits, kCertain);
+        const uint32_t most = largest_below(before);
+        if (r) certain &= ahead(before >> kIndexBits, most >> kIndexBits, apart);
         before = most;
 #pragma unroll
         for (uint32_t i = 0; i < kSlots; ++i) won[i] = sub + i * LANES == r ? most : won[i];
     }
     if (WORD != RouteWord::kLogit16) {
-        const uint32_t left = largest();
-        certain &= left == 0u || ahead(before >> kIndexBits, left >> kIndexBits, kCertain);
+        const uint32_t left = largest_below(before);
+        certain &= left >= before || ahead(before >> kIndexBits, left >> kIndexBits, apart);  // (not below: nothing is left)
     }
 
     // ---- the weights
@@ -520,6 +545,7 @@ extern "C" int shrike_hip_route_rows(void *stream, const shrike_route_desc *desc
     a.scaling = desc->scaling;
     const uint64_t size_of = logits_dtype == SHRIKE_ELEM_F32 ? 4u : 2u;
     a.whole = reinterpret_cast<uintptr_t>(d_logits) % 16u == 0 && (rows == 1u || logits_stride_elements * size_of % 16u == 0) && a.experts * size_of % 16u == 0;
+    a.whole_bias = d_bias && reinterpret_cast<uintptr_t>(d_bias) % 16u == 0 && a.experts * (bias_dtype == SHRIKE_ELEM_F32 ? 4u : 2u) % 16u == 0;
     constexpr uint32_t kMostRows = 1u << 24;  // of a launch, which holds fewer than 2^32 threads
     for (uint32_t done = 0; done < rows; done += kMostRows) {
         RouteArgs part = a;
