@@ -264,7 +264,8 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     constexpr int kWide = LANES * NPL < 64 ? 1 : LANES * NPL / 64;  // experts a lane where a wave has the row
     constexpr uint32_t kIndexBits = WORD == RouteWord::kLogit16 ? 16 : 10, kRows = 64 / LANES, kSlots = LANES == 16 ? 2 : 1;
     constexpr uint32_t kOutWord = WORD == RouteWord::kLogit16 ? 0 : 1;  // what an expert out of service has above its number
-    __shared__ double s_value[4][64 * kWide];
+    constexpr int kDoubles = 64 * kWide < int(kRows) * 64 ? int(kRows) * 64 : 64 * kWide;
+    __shared__ double s_value[4][kDoubles];
     const uint32_t lane = threadIdx.x & 63u, wave = wave_index(), sub = lane % LANES;
     const uint64_t first_row = (uint64_t(blockIdx.x) * 4u + wave) * kRows;
     if (first_row >= a.rows) return;
@@ -394,16 +395,75 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
         for (int j = 1; j < NPL; ++j) best = max(best, key[j] - taken);
         return lanes_max<LANES>(best) + taken;
     };
+    bool apart_all = true;
     for (uint32_t r = 0; r < a.top_k; ++r) {
         const uint32_t most = largest_below(before);
-        if (r) certain &= ahead(before >> kIndexBits, most >> kIndexBits, apart);
+        if (r) apart_all &= ahead(before >> kIndexBits, most >> kIndexBits, apart);
         before = most;
 #pragma unroll
         for (uint32_t i = 0; i < kSlots; ++i) won[i] = sub + i * LANES == r ? most : won[i];
     }
-    if (WORD != RouteWord::kLogit16) {
-        const uint32_t left = largest_below(before);
-        certain &= left >= before || ahead(before >> kIndexBits, left >> kIndexBits, apart);  // (not below: nothing is left)
+    uint32_t place[kSlots];  // in the route
+#pragma unroll
+    for (uint32_t i = 0; i < kSlots; ++i) place[i] = sub + i * LANES;
+    if constexpr (WORD != RouteWord::kLogit16) {
+        // Where words lie too close together, those that come next are taken too, up to a gap, and 64 bits put all that were taken into order: their
+        // scores alone, not the row's. (A softmax's sum stays the fp32 one: two choices whose difference it could turn are left to route_row.)
+        uint32_t left = largest_below(before), taken = a.top_k;
+        auto gap = [&] { return left >= before || ahead(before >> kIndexBits, left >> kIndexBits, apart); };  // (not below: nothing is left)
+        bool open = certain && !gap();
+        const bool closer = certain && (open || !apart_all);
+        if (__ballot(closer) != 0) {
+            while (__ballot(open) != 0) {
+                if (open && taken == 32u) {
+                    certain = open = false;
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < kSlots; ++i) won[i] = open && sub + i * LANES == taken ? left : won[i];
+                before = open ? left : before;
+                taken += open ? 1u : 0u;
+                left = largest_below(before);
+                open &= !gap();
+            }
+            double *const values = s_value[wave] + lane / LANES * 64u, *const scores = values + 32;
+            double mine[kSlots], my_score[kSlots];
+            uint32_t number[kSlots];
+#pragma unroll
+            for (uint32_t i = 0; i < kSlots; ++i) {
+                const uint32_t slot = sub + i * LANES;
+                number[i] = min(1023u - (won[i] & 0x3ffu), a.experts - 1u);
+                const float logit = in_service(route_load(a.logits, at + number[i], a.logits_type));
+                my_score[i] = !a.bias || logit == -INFINITY ? 0.0 : a.sigmoid ? 1.0 / (1.0 + exp(-double(logit))) : exp(double(logit) - double(base)) * double(inverse);
+                mine[i] = a.bias ? my_score[i] + double(in_service(route_load(a.bias, number[i], a.bias_type))) : double(logit);
+                if ((won[i] >> kIndexBits) <= kOutWord) mine[i] = -INFINITY;
+                if (slot < 32u) {
+                    values[slot] = mine[i];
+                    scores[slot] = my_score[i];
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+            uint32_t rank[kSlots] = {};
+            bool known = true;
+            for (uint32_t c = 0; c < 32u && __ballot(c < taken) != 0; ++c) {
+                const double v = values[c], of = scores[c];
+                const uint32_t e = 1023u - (__shfl(won[0], int(lane / LANES * LANES + c % LANES)) & 0x3ffu);
+                const uint32_t e2 = kSlots == 2 ? 1023u - (__shfl(won[kSlots - 1], int(lane / LANES * LANES + c % LANES)) & 0x3ffu) : e;
+                const uint32_t other = c < LANES ? e : e2;
+                if (c < taken)
+#pragma unroll
+                    for (uint32_t i = 0; i < kSlots; ++i) {
+                        rank[i] += v > mine[i] || (v == mine[i] && other < number[i]) ? 1u : 0u;
+                        if (!a.sigmoid && a.bias && sub + i * LANES < taken && v != mine[i] && v > -INFINITY && mine[i] > -INFINITY)
+                            known &= fabs(v - mine[i]) > fabs(of - my_score[i]) * 0x1p-20;
+                    }
+            }
+            __builtin_amdgcn_wave_barrier();
+            if (closer) {
+                certain &= lanes_max<LANES>(known ? 0u : 1u) == 0u;
+#pragma unroll
+                for (uint32_t i = 0; i < kSlots; ++i) place[i] = sub + i * LANES < taken ? rank[i] : ~0u;
+            }
+        }
     }
 
     // ---- the weights
@@ -412,7 +472,7 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     bool served[kSlots];
 #pragma unroll
     for (uint32_t i = 0; i < kSlots; ++i) {
-        const bool on = sub + i * LANES < a.top_k;
+        const bool on = place[i] < a.top_k;
         index[i] = on ? (WORD == RouteWord::kLogit16 ? 1024u - (won[i] & 0xffffu) : 1023u - (won[i] & 0x3ffu)) : 0u;
         served[i] = on && (won[i] >> kIndexBits) > kOutWord;
         w[i] = in_service(route_load(a.logits, at + min(index[i], a.experts - 1u), a.logits_type));
@@ -428,7 +488,7 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     if (a.renormalize) {
         sum = lanes_sum<LANES>(sum);
         // (scores that fp32 does not hold well are 64 bits' again; none in service leaves zeros)
-        if (a.sigmoid) certain &= sum > 1e-30f || lanes_max<LANES>(served[0] ? 1u : 0u) == 0u;
+        if (a.sigmoid) certain &= sum > 1e-30f || lanes_max<LANES>(served[0] || served[kSlots - 1] ? 1u : 0u) == 0u;
         const float factor = sum > 0.0f ? a.scaling / sum : 0.0f;
 #pragma unroll
         for (uint32_t i = 0; i < kSlots; ++i) w[i] *= factor;
@@ -439,9 +499,9 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     if (real && certain)
 #pragma unroll
         for (uint32_t i = 0; i < kSlots; ++i)
-            if (sub + i * LANES < a.top_k) {
-                a.indices[row * a.top_k + sub + i * LANES] = index[i];
-                route_store_weight(a, row * a.top_k + sub + i * LANES, double(w[i]));
+            if (place[i] < a.top_k) {
+                a.indices[row * a.top_k + place[i]] = index[i];
+                route_store_weight(a, row * a.top_k + place[i], double(w[i]));
             }
     // ---- rows that are not certain, one by one by the whole wave
     for (uint64_t again = __ballot(real && !certain && sub == 0); again; again &= again - 1u)
