@@ -26,7 +26,7 @@ __device__ __forceinline__ float route_load(const void *p, uint64_t i, uint32_t 
     return type == SHRIKE_ELEM_F16 ? f16_to_f32(h) : bf16_to_f32(h);
 }
 // NaN stands for -inf, +inf for the largest finite value
-__device__ __forceinline__ float in_service(float v) { return v != v ? -INFINITY : fminf(v, 3.4028234663852886e38f); }
+__device__ __forceinline__ float in_service(float v) { return fminf(fmaxf(v, -INFINITY), 3.4028234663852886e38f); }  // (fmaxf takes the number of a number and a NaN)
 
 __device__ __forceinline__ uint64_t order_key(double v) {
     const uint64_t u = uint64_t(__double_as_longlong(v + 0.0));  // -0 and +0 tie
@@ -282,19 +282,26 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
         uint16_t unused[NPL];
         if (a.bias) load_experts<NPL>(a.bias, 0, a.bias_type, a.whole_bias, sub, a.experts, b, unused);
     }
+    const bool full = a.experts == uint32_t(LANES * NPL);  // every lane's experts are there
     float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) {
-        l[j] = sub * NPL + j < a.experts ? in_service(l[j]) : -INFINITY;
-        top = fmaxf(top, l[j]);
-    }
+    for (int j = 0; j < NPL; ++j) l[j] = in_service(l[j]);
+    if (!full)
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) l[j] = sub * NPL + j < a.experts ? l[j] : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) top = fmaxf(top, l[j]);
     top = lanes_max<LANES>(top);
     const float base = top == -INFINITY ? 0.0f : top;
     float inverse = 0.0f;  // of the softmax's sum, where it is wanted
+    float v[NPL];
     if (!a.sigmoid && (WORD == RouteWord::kValue || !a.renormalize)) {
         float total = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) total += exp_fast(l[j] - base);
+        for (int j = 0; j < NPL; ++j) {
+            v[j] = exp_fast(l[j] - base);
+            total += v[j];
+        }
         total = lanes_sum<LANES>(total);
         inverse = total > 0.0f ? __builtin_amdgcn_rcpf(total) : 0.0f;
     }
@@ -310,12 +317,15 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
             key[j] = e >= a.experts ? 0u : (l[j] == -INFINITY ? 0u : order << 16) | (1024u - e);
         }
     } else {
-        float v[NPL], most = -INFINITY, least = INFINITY;
+        float most = -INFINITY, least = INFINITY;
+        if (WORD == RouteWord::kValue && a.sigmoid)
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) v[j] = score(l[j]);
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
-            v[j] = l[j];
+            if constexpr (WORD == RouteWord::kLogit) v[j] = l[j];
             if constexpr (WORD == RouteWord::kValue) {
-                float value = score(l[j]) + in_service(b[j]);
+                float value = fmaf(v[j], a.sigmoid ? 1.0f : inverse, in_service(b[j]));
                 asm volatile("" : "+v"(value));  // (or the compiler branches round it, lane by lane)
                 v[j] = l[j] == -INFINITY ? -INFINITY : value;
             }
@@ -331,14 +341,17 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
             const float off = (a.sigmoid ? 1.0f : inverse) * 0x1p-22f + (fabsf(most) + span) * 0x1p-24f;
             apart = 3u + uint32_t(2.0f * off * (kUnits / span));
         }
-        const float low = most - span, per_unit = kUnits / span;
+        const float per_unit = kUnits / span, from = -(most - span) * per_unit;
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
             const uint32_t e = sub * NPL + j;
             // 2: as far below the largest as the word reaches, or further
-            const uint32_t q = v[j] == -INFINITY ? kOutWord : min(max(uint32_t(fmaxf((v[j] - low) * per_unit, 0.0f)), 2u), 0x3fffffu);
-            key[j] = e >= a.experts ? 0u : q << 10 | (1023u - e);
+            const uint32_t q = v[j] == -INFINITY ? kOutWord : uint32_t(__builtin_amdgcn_fmed3f(fmaf(v[j], per_unit, from), 2.0f, 4194303.0f));
+            key[j] = q << 10 | (1023u - e);
         }
+        if (!full)
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) key[j] = sub * NPL + j < a.experts ? key[j] : 0u;
     }
     // a ahead of b for certain, by the parts above their numbers
     auto ahead = [&](uint32_t a_, uint32_t b_, uint32_t by) { return WORD == RouteWord::kLogit16 || b_ <= kOutWord || a_ >= b_ + by; };
