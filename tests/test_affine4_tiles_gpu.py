@@ -1,0 +1,114 @@
+"""shrike_hip_affine4_product over many rows: every shape of a workgroup's tile (64 x 128 outputs, 128 x 128, 256 x 256, taken as there are tiles enough
+for the device), at the numbers where one gives way to the next, with edges, chunks and lengths that do not fill them."""
+import numpy as np
+import pytest
+
+from shrike_amd import capi, runtime as rt
+from tests import affine4_reference as ref
+from tests.affine4_reference import BF16, F16, F32
+from tests.test_affine4_gpu import closely, exactly
+
+pytestmark = pytest.mark.gpu
+
+# rows and outputs: 200 tiles and more of 128 x 128; of 256 x 256
+MIDDLE = [(65, 25600), (129, 12700), (1700, 1900), (25473, 70)]
+LARGE = [(257, 25400), (3600, 3500), (25601, 450), (51100, 129)]
+
+
+@pytest.mark.parametrize("rows,n", MIDDLE + LARGE)
+@pytest.mark.parametrize("k,group", [(32, 32), (64, 64), (128, 128), (288, 32)])
+def test_edges(gpu, rows, n, k, group):
+    r = np.random.default_rng(rows + k)
+    exactly(r, rows, n, k, group, F16 if k % 3 else BF16, F32, meta=F16 if group == 32 else BF16, symmetric=k == 64, bias=k == 128)
+
+
+@pytest.mark.parametrize("rows,n", [(1700, 1900), (1800, 7200)])
+@pytest.mark.parametrize("k,group", [(64, 32), (96, 32), (128, 64), (160, 32), (192, 64), (256, 32), (320, 64), (384, 128), (448, 64), (480, 32), (512, 128), (544, 32), (576, 64), (640, 128),
+                                     (1024, 64), (1056, 32), (1088, 64), (1152, 128), (2304, 64)])
+def test_lengths(gpu, rows, n, k, group):
+    r = np.random.default_rng(rows + k)
+    exactly(r, rows, n, k, group, BF16 if k % 128 else F16, F32, meta=BF16 if k % 64 else F16)
+
+
+@pytest.mark.parametrize("rows,n", [(300, 500), (1700, 1900), (3600, 3500)])
+@pytest.mark.parametrize("x_type", [F16, BF16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("symmetric", [False, True])
+def test_types(gpu, rows, n, x_type, group, symmetric):
+    r = np.random.default_rng(rows + group)
+    for out_type, meta, bias, pad, x_pad in ((F16, F16, True, 5, 8), (BF16, BF16, False, 0, 64), (F32, BF16 if symmetric else F16, True, 8, 0)):
+        closely(r, rows, n, 640, group, x_type, out_type, meta, symmetric, bias, pad=pad, x_pad=x_pad)
+
+
+@pytest.mark.parametrize("rows,n", [(64, 25600), (65, 25472), (128, 25600), (129, 25472), (256, 25600), (257, 25344), (8, 4096), (9, 4096), (16, 16384), (17, 16352), (17, 16384), (33, 8192)])
+def test_where_one_shape_gives_way_to_the_next(gpu, rows, n):
+    r = np.random.default_rng(rows + n)
+    for group in (32, 64, 128):
+        exactly(r, rows, n, 384, group, F16, F32)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 20, 64, 70, 300])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_the_longest_rows(gpu, rows, group):
+    r = np.random.default_rng(rows)
+    exactly(r, rows, 40, 65536, group, F16, F32)
+    closely(r, rows, 24, 65536 - 128, group, BF16, F16)
+
+
+@pytest.mark.parametrize("rows,n", [(600, 65), (600, 11000), (3700, 3584)])
+def test_rows_past_4_gib_in_tiles(gpu, rows, n):
+    """Rows of x that a tile reaches by 32 bits from its first, 4 GiB and more behind the first tile's; outputs as far apart."""
+    r = np.random.default_rng(rows)
+    k = 128
+    w = ref.Weights(r, n, k, whole=True)
+    x = ref.whole_rows(r, rows, k, F16)
+    want = ref.encode(ref.decode(x, F16) @ w.values.T, F32)
+    stride = (1 << 33) // 2 // (rows - 1) // 8 * 8 + 1000  # the last row starts 8 GiB in
+    assert stride * 512 < 1 << 32
+    out_stride = stride + n
+    far_x, far_out = rt.DeviceBuffer(((rows - 1) * stride + k) * 2), rt.DeviceBuffer(((rows - 1) * out_stride + n) * 4)
+    for i in range(rows):
+        far_x.upload(x[i], i * stride * 2)
+    rt.affine4_product(far_x, F16, stride, *w.device(), w.meta, 64, None, far_out, F32, out_stride, rows, n, k)
+    rt.synchronize()
+    for i in range(rows):
+        assert np.array_equal(far_out.download(np.float32, n, i * out_stride * 4), want[i]), i
+
+
+def test_nan_stays_in_its_row_and_output_of_large_tiles(gpu):
+    r = np.random.default_rng(5)
+    rows, n, k = 3600, 3500, 256
+    w = ref.Weights(r, n, k, whole=True)
+    x = ref.whole_rows(r, rows, k, F16)
+    want = ref.decode(x, F16) @ w.values.T
+    bad_rows, bad_outputs = [0, 255, 256, 1801, 3599], [0, 31, 32, 1777, 3499]
+    for i, value in zip(bad_rows, (0x7E00, 0x7C00, 0xFC00, 0x7E00, 0x7C00)):
+        x[i, (i * 7) % k] = value
+    for i in bad_outputs:
+        w.scale_bits[i, i % 4] = 0x7FC0
+    got = ref.run(x, F16, w, None, F32)
+    assert np.isnan(got[:, bad_outputs]).all() and not np.isfinite(got[bad_rows]).any()
+    rest = np.setdiff1d(np.arange(rows), bad_rows)[:, None], np.setdiff1d(np.arange(n), bad_outputs)[None]
+    ref.assert_exact(got[rest], want[rest], F32)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 17, 70, 1700, 3600])
+def test_weights_used_by_calls_at_once_and_again(gpu, rows):
+    """The same call on two streams at once, over and over: the same bits."""
+    r = np.random.default_rng(rows)
+    n, k = 3500, 512
+    w = ref.Weights(r, n, k)
+    x, on = rt.dev(ref.encode(r.standard_normal((rows, k)), F16)), w.device()
+    streams, outs = [rt.Stream(), rt.Stream()], [rt.empty(rows * n * 2) for _ in range(2)]
+    first = None
+    for _ in range(4):
+        for s, out in zip(streams, outs):
+            out.fill(0xFF)
+        rt.synchronize()
+        for s, out in zip(streams, outs):
+            rt.affine4_product(x, F16, k, *on, w.meta, 64, None, out, F16, n, rows, n, k, s)
+        for s, out in zip(streams, outs):
+            s.synchronize()
+            bits = out.download(np.uint16, rows * n)
+            first = bits if first is None else first
+            assert np.array_equal(bits, first)
