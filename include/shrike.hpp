@@ -538,6 +538,25 @@ struct PrefillRoutedExpertWave {
     std::vector<shrike_routed_expert_block> blocks;
     int paddedRows = 0, tailRows = 0;
 };
+// Routes from any producer's logits; the reference's routers make theirs themselves.
+struct LogitRouter {
+    // of every expert, without groups; `groups`, `kept_groups` and `group_top` are the caller's to change
+    static shrike_route_desc description(uint32_t numExperts, uint32_t topK, uint32_t scores, bool renormalize, float scaling = 1.0f) {
+        return {numExperts, topK, scores, 1, 1, 1, renormalize ? 1u : 0u, scaling};
+    }
+    static void encode(Stream s, const shrike_route_desc &desc, const void *logits, uint32_t logitsType, uint64_t logitsStrideElements, const void *bias,
+                       uint32_t biasType, uint32_t *outIndices, void *outWeights, uint32_t weightsType, uint32_t rows) {
+        check(shrike_hip_route_rows(s, &desc, logits, logitsType, logitsStrideElements, bias, biasType, outIndices, outWeights, weightsType, rows));
+    }
+};
+// out = x . w^T (+ bias) for 4-bit rows with a scale and a bias a group
+struct AffineProduct {
+    static void encode(Stream s, const void *x, uint32_t xType, uint64_t xStrideElements, const shrike_projection &w, uint32_t metaType, uint32_t groupSize,
+                       const void *bias, void *out, uint32_t outType, uint64_t outStrideElements, uint32_t rows, uint32_t n, uint32_t k) {
+        check(shrike_hip_affine4_product(s, x, xType, xStrideElements, &w, metaType, groupSize, bias, out, outType, outStrideElements, rows, n, k));
+    }
+};
+
 // Blocks of 32 elements with a power-of-two scale (E4M3 or E2M1), and what is made of them; the reference has no such format.
 struct MicroscaledBlocks {
     static void quantize(Stream s, const void *src, uint32_t srcType, uint64_t srcStrideElements, uint32_t format, void *codes, void *scales,
