@@ -163,7 +163,7 @@ __device__ __forceinline__ float gemv_dot(const uint4 &w, const GemvSlice &x) {
     }
 }
 
-template <int XT, int NCH, bool ONCE>
+template <int XT, int NCH>
 __global__ __launch_bounds__(256) void k_affine4_gemv(Affine4Args a, uint32_t shift, uint32_t turns) {
     const uint32_t lane = threadIdx.x & 63u, wave = blockIdx.x * 4u + wave_index(), waves = gridDim.x * 4u;
     const uint32_t cpr = a.k / 32u, per_row = a.k / 2u, groups = a.k / a.group, lanes = 1u << shift, rows = 64u >> shift;
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(256) void k_affine4_gemv(Affine4Args a, uint32_t sh
                 for (int i = 0; i < NCH; ++i) {
                     const uint32_t c = min((segment * NCH + i) * lanes + col, cpr - 1u), g = c >> group_shift;
                     const u32x4_t *from = reinterpret_cast<const u32x4_t *>(codes) + c;
-                    const u32x4_t v = ONCE ? __builtin_nontemporal_load(from) : *from;
+                    const u32x4_t v = __builtin_nontemporal_load(from);  // (201,088 x 2,880: 67.5 us without the hint, 66.3 with it; weights that a cache holds: as fast)
                     w[r][i] = make_uint4(v.x, v.y, v.z, v.w);
                     s[r][i] = scales[g];
                     b[r][i] = biases[g];
@@ -235,9 +235,7 @@ static int launch_gemv(const Affine4Args &a, uint32_t shift, hipStream_t s) {
     const uint64_t batches = (a.n + kGemvBatch<NCH> * (64u >> shift) - 1u) / (kGemvBatch<NCH> * (64u >> shift)), groups_of_waves = (batches + 3u) / 4u;
     const uint32_t most = 256u * (NCH == 1 ? 5u : NCH <= 4 ? 3u : 2u), turns = uint32_t((groups_of_waves + most - 1u) / most);
     const uint32_t workgroups = uint32_t((groups_of_waves + turns - 1u) / turns);
-    // weights that no cache holds are read with the hint that they will not be wanted again
-    if (uint64_t(a.n) * a.k / 2u >= uint64_t(192) << 20) hipLaunchKernelGGL((k_affine4_gemv<XT, NCH, true>), dim3(workgroups), dim3(256), 0, s, a, shift, turns);
-    else hipLaunchKernelGGL((k_affine4_gemv<XT, NCH, false>), dim3(workgroups), dim3(256), 0, s, a, shift, turns);
+    hipLaunchKernelGGL((k_affine4_gemv<XT, NCH>), dim3(workgroups), dim3(256), 0, s, a, shift, turns);
     SHRIKE_HIP(hipGetLastError());
     return 0;
 }
@@ -535,14 +533,26 @@ __global__ __launch_bounds__(64 * kFewWaves, R8 == 4 ? 2 : 4) void k_affine4_few
     }
 }
 
+// The parts that share k: twice as many as long as the device still holds all workgroups at once (one a CU, as its LDS goes) and every part has a
+// unit. Another round costs what the halved k gives: 64 rows of 5,120 x 2,880 take 20 us in two parts (160 workgroups), 26 in four (320).
+template <int R8>
+static uint64_t few_workgroups(const Affine4Args &a, uint32_t parts) {
+    const uint32_t blocks = (a.n + 31u) / 32u, per = kFewWaves / parts;
+    return uint64_t((blocks + per - 1u) / per) * ((a.rows + 8u * R8 - 1u) / (8u * R8));
+}
+template <int R8>
+static uint32_t few_parts(const Affine4Args &a) {
+    const uint32_t units = (a.k + kFewUnit - 1u) / kFewUnit;
+    uint32_t parts = 1;
+    while (parts < kFewWaves && FewLds<R8>::bytes(2u * parts) <= 160u * 1024u && parts * 2u <= units && few_workgroups<R8>(a, 2u * parts) <= 256u) parts *= 2u;
+    return parts;
+}
 template <int XT, int GROUP, int R8>
 static int launch_few(const Affine4Args &args, hipStream_t s) {
     typedef FewLds<R8> L;
     Affine4Args a = args;
-    const uint32_t blocks = (a.n + 31u) / 32u, tiles = (a.rows + 8u * R8 - 1u) / (8u * R8), units = (a.k + kFewUnit - 1u) / kFewUnit;
-    a.parts = 1;
-    while (a.parts < 8u && L::bytes(2u * a.parts) <= 160u * 1024u && a.parts * 2u <= units && uint64_t(blocks) * tiles * a.parts < 8u * 256u) a.parts *= 2u;
-    const uint32_t bytes = L::bytes(a.parts);
+    a.parts = few_parts<R8>(a);
+    const uint32_t blocks = (a.n + 31u) / 32u, tiles = (a.rows + 8u * R8 - 1u) / (8u * R8), bytes = L::bytes(a.parts);
     static_assert(kFewWaves * 4u * R8 * 256u <= L::bytes(1), "the parts' sums fit");
     const uint32_t per = kFewWaves / a.parts;
     hipLaunchKernelGGL((k_affine4_few<XT, GROUP, R8>), dim3((blocks + per - 1u) / per, tiles), dim3(64u * kFewWaves), bytes, s, a);
@@ -791,7 +801,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS, 2) void k_affine4_tile(Affine4Ar
             for (int i = 0; i < NT; ++i) factors[c][i] = meta_f32(next_scales[c][i], a.meta);
         auto slots = [&](auto slot_) {  // an instruction and what stands behind it
             constexpr int slot = decltype(slot_)::value, j = slot % kPer, chain = slot / kPer, i = chain % NT, c = chain / NT % kSubs, m = chain / NT / kSubs;
-            constexpr int chains = MT * kSubs * NT, last = (chain + chains - 1) % chains, next = (chain + 1) % chains, at = c * kPer + j;
+            constexpr int chains = MT * kSubs * NT, last = (chain + chains - 1) % chains, at = c * kPer + j;
             f32x16 &now = p[kBehind ? chain & 1 : 0], &old = p[kBehind ? (chain & 1) ^ 1 : 0];
             f32x16 &into = acc[last / NT / kSubs][last % NT];
             if constexpr (j == 0) {
@@ -1012,17 +1022,37 @@ static int launch_tile(const Affine4Args &a, hipStream_t s) {
     return 0;
 }
 
+// Which shape: the one that takes the least by its rounds (of 256 workgroups, one a CU), the units of 256 k a round, and what a unit takes, in
+// parts of half a microsecond: 3 for 8 rows x 256 outputs, 4 for 16 x 256, 6 for 32 x 256, 8 for a tile of 128 x 128, 22 for 256 x 256. Measured, in us:
+//   rows x n x k              8 rows   16 rows   32 rows   128 x 128   256 x 256
+//   16 x 4,096 x 4,096          10.7      17.2      25.2        53.5       141.9
+//   64 x 8,192 x 2,048          18.2      14.5      18.6        30.7        75.7
+//   64 x 16,384 x 2,304         31.4      24.1      22.7        38.3        85.3
+//   128 x 4,096 x 4,096         33.3      24.8      31.4        55.6       148.1
+//   300 x 4,096 x 2,048         39.0      38.9      24.6        33.3        79.5
+//   512 x 8,192 x 2,048         94.0      77.6      49.3        35.2        80.4
+//   2,048 x 4,096 x 4,096      370.2     284.9     176.6       116.5       148.8
+//   2,048 x 6,144 x 4,096      547.5     410.9     261.3       172.0       153.7
+//   4,096 x 5,120 x 2,048      449.4     372.6     228.0       162.9       166.0
+template <int R8>
+static uint64_t few_cost(const Affine4Args &a) {
+    const uint32_t parts = few_parts<R8>(a), units = (a.k + kFewUnit - 1u) / kFewUnit;
+    return (few_workgroups<R8>(a, parts) + 255u) / 256u * ((units + parts - 1u) / parts) * (R8 == 4 ? 6u : R8 == 2 ? 4u : 3u);
+}
+static uint64_t tile_cost(const Affine4Args &a, uint32_t side, uint32_t cost) {
+    const uint64_t tiles = uint64_t((a.rows + side - 1u) / side) * ((a.n + side - 1u) / side);
+    return (tiles + 255u) / 256u * ((a.k + kFewUnit - 1u) / kFewUnit) * cost;
+}
 template <int XT, int GROUP>
 static int launch_affine4(const Affine4Args &a, hipStream_t s) {
     if (a.rows <= 8u) return launch_few<XT, GROUP, 1>(a, s);
-    if (a.rows > 64u && a.x_stride * 512u < uint64_t(1) << 32) {  // (a tile's rows are reached by 32 bits)
-        if (uint64_t((a.n + 255u) / 256u) * ((a.rows + 255u) / 256u) >= 200u) return launch_tile<XT, GROUP, 4, 2, 2, 4, 3, 1>(a, s);
-        if (uint64_t((a.n + 127u) / 128u) * ((a.rows + 127u) / 128u) >= 200u) return launch_tile<XT, GROUP, 4, 1, 1, 4, 3, 2>(a, s);
-        return launch_tile<XT, GROUP, 2, 1, 1, 4, 4, 2>(a, s);
+    const uint64_t few[3] = {few_cost<1>(a), few_cost<2>(a), few_cost<4>(a)}, least = std::min(few[0], std::min(few[1], few[2]));
+    if (a.x_stride * 512u < uint64_t(1) << 32) {  // (a tile's rows are reached by 32 bits)
+        const uint64_t tile = tile_cost(a, 128, 8), large = tile_cost(a, 256, 22);
+        if (std::min(tile, large) < least) return tile <= large ? launch_tile<XT, GROUP, 4, 1, 1, 4, 3, 2>(a, s) : launch_tile<XT, GROUP, 4, 2, 2, 4, 3, 1>(a, s);
     }
-    const uint64_t blocks = (a.n + 31u) / 32u;
-    if (a.rows <= 16u || blocks * ((a.rows + 31u) / 32u) < 512u) return launch_few<XT, GROUP, 2>(a, s);
-    return launch_few<XT, GROUP, 4>(a, s);
+    if (few[1] == least) return launch_few<XT, GROUP, 2>(a, s);
+    return few[2] == least ? launch_few<XT, GROUP, 4>(a, s) : launch_few<XT, GROUP, 1>(a, s);
 }
 template <int XT>
 static int launch_affine4(const Affine4Args &a, hipStream_t s) {

@@ -1,5 +1,5 @@
-"""shrike_hip_affine4_product over many rows: every shape of a workgroup's tile (64 x 128 outputs, 128 x 128, 256 x 256, taken as there are tiles enough
-for the device), at the numbers where one gives way to the next, with edges, chunks and lengths that do not fill them."""
+"""shrike_hip_affine4_product over many rows: every shape of a workgroup (8, 16 or 32 rows with k in parts, tiles of 128 x 128 and of 256 x 256 outputs,
+taken as there is work for the device), about where one gives way to the next, with edges, chunks and lengths that do not fill them."""
 import numpy as np
 import pytest
 
@@ -10,8 +10,8 @@ from tests.test_affine4_gpu import closely, exactly
 
 pytestmark = pytest.mark.gpu
 
-# rows and outputs: 200 tiles and more of 128 x 128; of 256 x 256
-MIDDLE = [(65, 25600), (129, 12700), (1700, 1900), (25473, 70)]
+# rows and outputs: more than two workgroups a CU of 32 rows x 256 outputs, no more than 256 tiles of 128 x 128; more than 512 of those
+MIDDLE = [(65, 25600), (130, 16000), (1700, 1900), (25473, 70)]
 LARGE = [(257, 25400), (3600, 3500), (25601, 450), (51100, 129)]
 
 
@@ -40,7 +40,9 @@ def test_types(gpu, rows, n, x_type, group, symmetric):
         closely(r, rows, n, 640, group, x_type, out_type, meta, symmetric, bias, pad=pad, x_pad=x_pad)
 
 
-@pytest.mark.parametrize("rows,n", [(64, 25600), (65, 25472), (128, 25600), (129, 25472), (256, 25600), (257, 25344), (8, 4096), (9, 4096), (16, 16384), (17, 16352), (17, 16384), (33, 8192)])
+@pytest.mark.parametrize("rows,n", [(8, 4096), (9, 4096), (9, 40000), (16, 8192), (17, 8192), (16, 16384), (17, 16384), (33, 8192), (33, 16384), (64, 16384), (65, 16384), (64, 25600),
+                                    (65, 25472), (128, 25600), (129, 25472), (512, 4096), (513, 4096), (512, 4097), (512, 8192), (513, 8192), (2048, 4096), (2048, 4097), (2049, 4096),
+                                    (256, 65536), (257, 65536), (4096, 4352), (20000, 32), (20000, 200), (9, 32), (65, 1), (1000, 33), (5000, 40)])
 def test_where_one_shape_gives_way_to_the_next(gpu, rows, n):
     r = np.random.default_rng(rows + n)
     for group in (32, 64, 128):
@@ -55,7 +57,7 @@ def test_the_longest_rows(gpu, rows, group):
     closely(r, rows, 24, 65536 - 128, group, BF16, F16)
 
 
-@pytest.mark.parametrize("rows,n", [(600, 65), (600, 11000), (3700, 3584)])
+@pytest.mark.parametrize("rows,n", [(600, 5000), (600, 11000), (3700, 3584)])
 def test_rows_past_4_gib_in_tiles(gpu, rows, n):
     """Rows of x that a tile reaches by 32 bits from its first, 4 GiB and more behind the first tile's; outputs as far apart."""
     r = np.random.default_rng(rows)
