@@ -279,7 +279,11 @@ __device__ __forceinline__ uint4 affine4_load16(buffer_t b, uint32_t at, uint32_
 //
 // Up to 8 R8 rows a workgroup of eight waves; `parts` of them share an output block's k, the others have blocks of their own. A wave's
 // block is 32 outputs, a lane's column of it one output. Codes and rows come through LDS, a unit of 256 k (four steps, a line of a row of codes)
-// ahead, the codes a wave's own, the rows a part's. While a unit is multiplied, the group sums of its rows are formed beside it, and the bias term of the unit before is added.
+// ahead, the rows a part's in two places, the codes a wave's own in one: they go on into registers before the next are asked for. While a unit is
+// multiplied, the group sums of its rows are formed beside it, and the bias term of the unit before is added. What bounds it is the issue of
+// instructions: of some 300 a unit and wave 144 take the codes apart, and only 16 multiply. (Two sets of sums, so that one chain is scaled while the
+// next is multiplied, took the registers of two waves and 3 us more of 22; two copies of the loop for the scales of two units no less time.)
+// 8 rows of 5,120 x 2,880: 9.5 us; 37 of 2,049 x 2,304: 9.8; 64 of 16,384 x 2,304: 22 (1.0 TB/s of weights, 220 TFLOP/s).
 //
 // In a step lane half h has k = 32 h + 0..31 of both operands (groups of 32: 16 h + 0..15 of either group).
 
@@ -290,11 +294,11 @@ struct FewLds {
     static constexpr uint32_t kSums = 8u * R8 * 48u;         // their sums: three terms of up to eight groups
     static constexpr uint32_t kPart = 2u * (kX + kSums);     // two places
     static constexpr uint32_t kCodes = 32u * kFewUnit / 2u;  // a wave's codes of a unit
-    static constexpr uint32_t bytes(uint32_t parts) { return parts * kPart + kFewWaves * 2u * kCodes; }
+    static constexpr uint32_t bytes(uint32_t parts) { return parts * kPart + kFewWaves * kCodes; }
 };
 
 template <int XT, int GROUP, int R8>
-__global__ __launch_bounds__(64 * kFewWaves, R8 == 4 ? 2 : 4) void k_affine4_few(Affine4Args a) {
+__global__ __launch_bounds__(64 * kFewWaves, 2) void k_affine4_few(Affine4Args a) {
     typedef FewLds<R8> L;
     constexpr bool SUB32 = GROUP == 32;
     constexpr int kRegs = 4 * R8;  // of a 32 x 32 block, those of the rows there are
@@ -326,11 +330,11 @@ __global__ __launch_bounds__(64 * kFewWaves, R8 == 4 ? 2 : 4) void k_affine4_few
     // once; past k stands the row's last piece.
     constexpr uint32_t kStepX = 8u * R8 * 128u;
     auto load_x = [&](uint32_t u) {
-        const uint32_t eights = (rows + 7u) / 8u, swizzled = lane & 7u, r8 = lane >> 3;
-        for (uint32_t i = wave; i < a.parts * 4u * eights; i += kFewWaves) {
-            const uint32_t s = i & 3u, p = (i >> 2) / eights, r = 8u * ((i >> 2) - p * eights) + r8;
+        const uint32_t swizzled = lane & 7u, r8 = lane >> 3;
+        for (uint32_t i = wave; i < a.parts * 4u * R8; i += kFewWaves) {
+            const uint32_t s = i & 3u, p = (i >> 2) / R8, eight = (i >> 2) % R8, r = 8u * eight + r8;
             const uint32_t piece = (p * rounds + u) * (kFewUnit / 8u) + 8u * s;
-            if (piece >= pieces) continue;
+            if (8u * eight >= rows || piece >= pieces) continue;
             lds_load16(lds0 + x_place(p, u) + s * kStepX + (r - r8) * 128u,
                        a.x + uint64_t(row0 + min(r, rows - 1u)) * a.x_stride + min(piece + (swizzled ^ ((r >> 1) & 7u)), pieces - 1u) * 8u);
         }
@@ -341,7 +345,7 @@ __global__ __launch_bounds__(64 * kFewWaves, R8 == 4 ? 2 : 4) void k_affine4_few
 
     // The wave's codes of unit u into its place: a line (128 bytes) of eight rows a load, eight lanes a row, xor-ed as the rows of x are; past
     // the row's end stands its last piece.
-    const uint32_t lds_codes = a.parts * L::kPart + wave * 2u * L::kCodes;
+    const uint32_t lds_codes = a.parts * L::kPart + wave * L::kCodes;
     const uint32_t code_pieces = a.k / 32u, line_piece = (lane & 7u) ^ (lane >> 4);  // (xor-ed with 4 in every second load)
     uint32_t line_at[4];
 #pragma unroll
@@ -350,7 +354,7 @@ __global__ __launch_bounds__(64 * kFewWaves, R8 == 4 ? 2 : 4) void k_affine4_few
         uint32_t s[kChains / 2], b[kChains / 2];
     };
     auto load_unit = [&](Unit &t, uint32_t u) {
-        const uint32_t unit = first + u, to = lds0 + lds_codes + (u & 1u) * L::kCodes;
+        const uint32_t unit = first + u, to = lds0 + lds_codes;
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j)
             lds_load16(to + j * 1024u, codes, line_at[j] + min(unit * 8u + (line_piece ^ (4u * (j & 1u))), code_pieces - 1u) * 16u);
@@ -391,14 +395,12 @@ __global__ __launch_bounds__(64 * kFewWaves, R8 == 4 ? 2 : 4) void k_affine4_few
 
     const uint32_t my_row = min(col, rows - 1u);  // the row of LDS that a lane's row of the operand is (rows past the last: the last)
 
-    auto multiply = [&](const Unit &t, uint32_t u, auto whole) {
+    auto multiply = [&](const Unit &t, const uint4 (&codes)[4], uint32_t u, auto whole) {
         const uint32_t left = decltype(whole)::value ? kFewUnit : a.k - (first + u) * kFewUnit;  // of the row, from this unit on
-        const uint8_t *const my_codes = lds + lds_codes + (u & 1u) * L::kCodes + col * 128u;
 #pragma unroll
         for (uint32_t s = 0; s < 4; ++s) {
             if (64u * s >= left) break;
-            const uint4 v = *reinterpret_cast<const uint4 *>(my_codes + (((2u * s + half) ^ ((col >> 1) & 7u)) * 16u));
-            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            uint32_t w[4] = {codes[s].x, codes[s].y, codes[s].z, codes[s].w};
             if constexpr (SUB32) {
                 // lane half h has group h of the step: its halves to both (past the row's end there is no second group)
                 if (64u * s + 32u >= left)
@@ -432,8 +434,9 @@ __global__ __launch_bounds__(64 * kFewWaves, R8 == 4 ? 2 : 4) void k_affine4_few
     };
     // The group sums of every part's unit u, as three bf16 terms of each: a lane a piece, eight lanes (four) a group.
     auto form_sums = [&](uint32_t u) {
-        for (uint32_t i = threadIdx.x; i < a.parts * rows * 32u; i += 64u * kFewWaves) {
-            const uint32_t piece = i % 32u, r = i / 32u % rows, p = i / 32u / rows, at = (p * rounds + u) * kFewUnit + 8u * piece;
+        for (uint32_t i = threadIdx.x; i < a.parts * 256u * R8; i += 64u * kFewWaves) {
+            const uint32_t piece = i % 32u, r = i / 32u % (8u * R8), p = i / (256u * R8), at = (p * rounds + u) * kFewUnit + 8u * piece;
+            if (r >= rows) continue;
             float sum = affine4_add<XT>(read_x(x_place(p, u), piece / 8u, r, piece % 8u), 0.0f);
             sum = at < a.k ? sum : 0.0f;
             sum = __fadd_rn(sum, dpp_f32<0xB1>(sum));
@@ -483,28 +486,30 @@ __global__ __launch_bounds__(64 * kFewWaves, R8 == 4 ? 2 : 4) void k_affine4_few
         for (int r = 0; r < kRegs; ++r) acc[r] = __fadd_rn(acc[r], p[r]);
     };
 
-    Unit t[2];
+    Unit next;
     uint32_t kept[kChains / 2];  // the biases of the unit before
     load_x(0);
-    if (active && mine) load_unit(t[0], 0);
-    auto phase = [&](Unit &now, Unit &next, uint32_t u) {
+    if (active && mine) load_unit(next, 0);
+    for (uint32_t u = 0; u < rounds; ++u) {
         // all that the unit needs has landed, for every wave; and nobody reads the places of the one before any more
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), in the compiler's own count too
         wait_loads_and_sync<0>();
+        const Unit now = next;
+        // the unit's codes into registers, and the next ones into their place
+        uint4 raw[4];
+#pragma unroll
+        for (uint32_t s = 0; s < 4; ++s) raw[s] = *reinterpret_cast<const uint4 *>(lds + lds_codes + col * 128u + (((2u * s + half) ^ ((col >> 1) & 7u)) * 16u));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (u + 1u < rounds) load_x(u + 1u);
         if (active && u + 1u < mine) load_unit(next, u + 1u);
         form_sums(u);
         if (active && u && u - 1u < mine) add_bias(kept, u - 1u);
         if (active && u < mine) {
-            if ((first + u + 1u) * kFewUnit <= a.k) multiply(now, u, std::true_type{});
-            else multiply(now, u, std::false_type{});
+            if ((first + u + 1u) * kFewUnit <= a.k) multiply(now, raw, u, std::true_type{});
+            else multiply(now, raw, u, std::false_type{});
 #pragma unroll
             for (uint32_t j = 0; j < kChains / 2u; ++j) kept[j] = now.b[j];
         }
-    };
-    for (uint32_t u = 0; u < rounds; u += 2u) {
-        phase(t[0], t[1], u);
-        if (u + 1u < rounds) phase(t[1], t[0], u + 1u);
     }
     __syncthreads();
     if (active && mine == rounds) add_bias(kept, rounds - 1u);
@@ -533,8 +538,8 @@ __global__ __launch_bounds__(64 * kFewWaves, R8 == 4 ? 2 : 4) void k_affine4_few
     }
 }
 
-// The parts that share k: twice as many as long as the device still holds all workgroups at once (one a CU, as its LDS goes) and every part has a
-// unit. Another round costs what the halved k gives: 64 rows of 5,120 x 2,880 take 20 us in two parts (160 workgroups), 26 in four (320).
+// The parts that share k: twice as many as long as every CU has at most one workgroup and every part a unit. A second one costs what the halved k gives:
+// 64 rows of 5,120 x 2,880 take 20 us in two parts (160 workgroups), 26 in four (320).
 template <int R8>
 static uint64_t few_workgroups(const Affine4Args &a, uint32_t parts) {
     const uint32_t blocks = (a.n + 31u) / 32u, per = kFewWaves / parts;
@@ -1025,11 +1030,11 @@ static int launch_tile(const Affine4Args &a, hipStream_t s) {
 // Which shape: the one that takes the least by its rounds (of 256 workgroups, one a CU), the units of 256 k a round, and what a unit takes, in
 // parts of half a microsecond: 3 for 8 rows x 256 outputs, 4 for 16 x 256, 6 for 32 x 256, 8 for a tile of 128 x 128, 22 for 256 x 256. Measured, in us:
 //   rows x n x k              8 rows   16 rows   32 rows   128 x 128   256 x 256
-//   16 x 4,096 x 4,096          10.7      17.2      25.2        53.5       141.9
-//   64 x 8,192 x 2,048          18.2      14.5      18.6        30.7        75.7
-//   64 x 16,384 x 2,304         31.4      24.1      22.7        38.3        85.3
-//   128 x 4,096 x 4,096         33.3      24.8      31.4        55.6       148.1
-//   300 x 4,096 x 2,048         39.0      38.9      24.6        33.3        79.5
+//   16 x 4,096 x 4,096           9.7      15.8      27.0        53.5       141.9
+//   64 x 8,192 x 2,048          18.7      14.3      18.8        30.7        75.7
+//   64 x 16,384 x 2,304         30.5      22.7      22.1        38.3        85.3
+//   128 x 4,096 x 4,096         31.5      22.9      31.1        55.6       148.1
+//   300 x 4,096 x 2,048         37.3      28.1      24.9        33.3        79.5
 //   512 x 8,192 x 2,048         94.0      77.6      49.3        35.2        80.4
 //   2,048 x 4,096 x 4,096      370.2     284.9     176.6       116.5       148.8
 //   2,048 x 6,144 x 4,096      547.5     410.9     261.3       172.0       153.7
