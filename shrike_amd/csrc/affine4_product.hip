@@ -1027,8 +1027,8 @@ static int launch_tile(const Affine4Args &a, hipStream_t s) {
     return 0;
 }
 
-// Which shape: the one that takes the least by its rounds (of 256 workgroups, one a CU), the units of 256 k a round, and what a unit takes, in
-// parts of half a microsecond: 3 for 8 rows x 256 outputs, 4 for 16 x 256, 6 for 32 x 256, 8 for a tile of 128 x 128, 22 for 256 x 256. Measured, in us:
+// Which shape: the one that takes the least, in tenths of a microsecond, by its rounds (of 256 workgroups), the units of 256 k a round, and what a unit,
+// a round and the call take. Measured, in us:
 //   rows x n x k              8 rows   16 rows   32 rows   128 x 128   256 x 256
 //   16 x 4,096 x 4,096           9.7      15.8      27.0        53.5       141.9
 //   64 x 8,192 x 2,048          18.7      14.3      18.8        30.7        75.7
@@ -1039,21 +1039,25 @@ static int launch_tile(const Affine4Args &a, hipStream_t s) {
 //   2,048 x 4,096 x 4,096      370.2     284.9     176.6       116.5       148.8
 //   2,048 x 6,144 x 4,096      547.5     410.9     261.3       172.0       153.7
 //   4,096 x 5,120 x 2,048      449.4     372.6     228.0       162.9       166.0
+//   513 x 26,428 x 320          86.9      53.6      39.3        80.5        54.6
+//   1,724 x 2,822 x 1,216       88.2      56.0      40.1        65.0        68.4
+//   3,108 x 14,040 x 64        139.7      91.3      63.4       111.4        53.8
 template <int R8>
 static uint64_t few_cost(const Affine4Args &a) {
-    const uint32_t parts = few_parts<R8>(a), units = (a.k + kFewUnit - 1u) / kFewUnit;
-    return (few_workgroups<R8>(a, parts) + 255u) / 256u * ((units + parts - 1u) / parts) * (R8 == 4 ? 6u : R8 == 2 ? 4u : 3u);
+    const uint32_t parts = few_parts<R8>(a), units = (a.k + kFewUnit - 1u) / kFewUnit, each = (units + parts - 1u) / parts;
+    const uint64_t rounds = (few_workgroups<R8>(a, parts) + 255u) / 256u;
+    return R8 == 1 ? rounds * each * 15u + 60u : R8 == 2 ? rounds * each * 20u + 60u : rounds * (each * 26u + 8u) + 50u;
 }
-static uint64_t tile_cost(const Affine4Args &a, uint32_t side, uint32_t cost) {
+static uint64_t tile_cost(const Affine4Args &a, uint32_t side, uint32_t unit, uint32_t call) {
     const uint64_t tiles = uint64_t((a.rows + side - 1u) / side) * ((a.n + side - 1u) / side);
-    return (tiles + 255u) / 256u * ((a.k + kFewUnit - 1u) / kFewUnit) * cost;
+    return (tiles + 255u) / 256u * ((a.k + kFewUnit - 1u) / kFewUnit * unit + 70u) + call;
 }
 template <int XT, int GROUP>
 static int launch_affine4(const Affine4Args &a, hipStream_t s) {
     if (a.rows <= 8u) return launch_few<XT, GROUP, 1>(a, s);
     const uint64_t few[3] = {few_cost<1>(a), few_cost<2>(a), few_cost<4>(a)}, least = std::min(few[0], std::min(few[1], few[2]));
     if (a.x_stride * 512u < uint64_t(1) << 32) {  // (a tile's rows are reached by 32 bits)
-        const uint64_t tile = tile_cost(a, 128, 8), large = tile_cost(a, 256, 22);
+        const uint64_t tile = tile_cost(a, 128, 29, 50), large = tile_cost(a, 256, 90, 100);
         if (std::min(tile, large) < least) return tile <= large ? launch_tile<XT, GROUP, 4, 1, 1, 4, 3, 2>(a, s) : launch_tile<XT, GROUP, 4, 2, 2, 4, 3, 1>(a, s);
     }
     if (few[1] == least) return launch_few<XT, GROUP, 2>(a, s);

@@ -17,7 +17,8 @@ struct RouteArgs {
     uint32_t rows, experts, top_k, groups, kept, group_size;
     uint32_t logits_type, bias_type, weights_type, group_top, sigmoid, renormalize;
     float scaling;
-    uint32_t whole, whole_bias;  // rows (the bias) start at multiples of 16 bytes and are multiples of 16 bytes long
+    uint32_t group_shift;        // 2^i lanes have a group
+    uint32_t whole, whole_bias;  // rows (the bias) and their groups start at multiples of 16 bytes and are multiples of 16 bytes long
 };
 
 __device__ __forceinline__ float route_load(const void *p, uint64_t i, uint32_t type) {
@@ -216,24 +217,24 @@ __device__ __forceinline__ float lanes_sum(float v) {
 }
 __device__ __forceinline__ float exp_fast(float v) { return __builtin_amdgcn_exp2f(1.4426950408889634f * v); }
 
-// NPL neighbouring values from `at` on for the sub-th lane of a row, and their 16 bits where they have 16; past the last expert something. `whole`: from 16-byte
-// aligned addresses, in whole loads.
+// NPL neighbouring values, from the expert `first` of the row at `at` on, and their 16 bits where they have 16; past the last expert something. `whole`: from
+// 16-byte aligned addresses, in whole loads.
 template <int NPL>
-__device__ __forceinline__ void load_experts(const void *from, uint64_t at, uint32_t type, uint32_t whole, uint32_t sub, uint32_t experts, float (&v)[NPL],
+__device__ __forceinline__ void load_experts(const void *from, uint64_t at, uint32_t type, uint32_t whole, uint32_t first, uint32_t experts, float (&v)[NPL],
                                              uint16_t (&bits)[NPL]) {
     if (type == SHRIKE_ELEM_F32) {
         const float *p = static_cast<const float *>(from) + at;
         if (NPL % 4 == 0 && whole) {
 #pragma unroll
             for (int j = 0; j < NPL; j += 4) {
-                const float4 f = *reinterpret_cast<const float4 *>(p + (sub * NPL + j < experts ? sub * NPL + j : 0u));
+                const float4 f = *reinterpret_cast<const float4 *>(p + (first + j < experts ? first + j : 0u));
                 const float w[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[(j + i) % NPL] = w[i];
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < NPL; ++j) v[j] = p[min(sub * NPL + j, experts - 1u)];
+            for (int j = 0; j < NPL; ++j) v[j] = p[min(first + j, experts - 1u)];
         }
         return;
     }
@@ -241,14 +242,14 @@ __device__ __forceinline__ void load_experts(const void *from, uint64_t at, uint
     if (NPL % 8 == 0 && whole) {
 #pragma unroll
         for (int j = 0; j < NPL; j += 8) {
-            const uint4 f = *reinterpret_cast<const uint4 *>(p + (sub * NPL + j < experts ? sub * NPL + j : 0u));
+            const uint4 f = *reinterpret_cast<const uint4 *>(p + (first + j < experts ? first + j : 0u));
             const uint32_t w[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) bits[(j + i) % NPL] = uint16_t(w[i / 2] >> 16 * (i % 2));
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) bits[j] = p[min(sub * NPL + j, experts - 1u)];
+        for (int j = 0; j < NPL; ++j) bits[j] = p[min(first + j, experts - 1u)];
     }
     if (type == SHRIKE_ELEM_F16) {
 #pragma unroll
@@ -272,15 +273,17 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     const bool real = first_row + lane / LANES < a.rows;
     const uint64_t row = real ? first_row + lane / LANES : a.rows - 1u, at = row * a.stride;
 
-    // ---- the row
+    // ---- the row: of 2^group_shift lanes a group's experts, up to NPL of them a lane
+    const uint32_t group = sub >> a.group_shift, within = (sub & ((1u << a.group_shift) - 1u)) * NPL, first = group * a.group_size + within;
+    const uint32_t have = group < a.groups && within < a.group_size ? a.group_size - within : 0u;  // (NPL or more: all of a lane's)
     float l[NPL], b[NPL];
     uint16_t bits[NPL];  // 16-bit logits as they are
-    load_experts<NPL>(a.logits, at, a.logits_type, a.whole, sub, a.experts, l, bits);
+    load_experts<NPL>(a.logits, at, a.logits_type, a.whole, first, a.experts, l, bits);
     if (WORD == RouteWord::kValue) {
 #pragma unroll
         for (int j = 0; j < NPL; ++j) b[j] = 0.0f;
         uint16_t unused[NPL];
-        if (a.bias) load_experts<NPL>(a.bias, 0, a.bias_type, a.whole_bias, sub, a.experts, b, unused);
+        if (a.bias) load_experts<NPL>(a.bias, 0, a.bias_type, a.whole_bias, first, a.experts, b, unused);
     }
     const bool full = a.experts == uint32_t(LANES * NPL);  // every lane's experts are there
     float top = -INFINITY;
@@ -288,7 +291,7 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     for (int j = 0; j < NPL; ++j) l[j] = in_service(l[j]);
     if (!full)
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) l[j] = sub * NPL + j < a.experts ? l[j] : -INFINITY;
+        for (uint32_t j = 0; j < NPL; ++j) l[j] = j < have ? l[j] : -INFINITY;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) top = fmaxf(top, l[j]);
     top = lanes_max<LANES>(top);
@@ -313,8 +316,8 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     if constexpr (WORD == RouteWord::kLogit16) {
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
-            const uint32_t e = sub * NPL + j, as_is = bits[j] == 0x8000u ? 0u : bits[j], order = (as_is & 0x8000u ? ~as_is : as_is | 0x8000u) & 0xffffu;
-            key[j] = e >= a.experts ? 0u : (l[j] == -INFINITY ? 0u : order << 16) | (1024u - e);
+            const uint32_t e = first + j, as_is = bits[j] == 0x8000u ? 0u : bits[j], order = (as_is & 0x8000u ? ~as_is : as_is | 0x8000u) & 0xffffu;
+            key[j] = j >= have ? 0u : (l[j] == -INFINITY ? 0u : order << 16) | (1024u - e);
         }
     } else {
         float most = -INFINITY, least = INFINITY;
@@ -344,21 +347,21 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
         const float per_unit = kUnits / span, from = -(most - span) * per_unit;
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
-            const uint32_t e = sub * NPL + j;
+            const uint32_t e = first + j;
             // 2: as far below the largest as the word reaches, or further
             const uint32_t q = v[j] == -INFINITY ? kOutWord : uint32_t(__builtin_amdgcn_fmed3f(fmaf(v[j], per_unit, from), 2.0f, 4194303.0f));
             key[j] = q << 10 | (1023u - e);
         }
         if (!full)
 #pragma unroll
-            for (int j = 0; j < NPL; ++j) key[j] = sub * NPL + j < a.experts ? key[j] : 0u;
+            for (int j = 0; j < NPL; ++j) key[j] = j < have ? key[j] : 0u;
     }
     // a ahead of b for certain, by the parts above their numbers
     auto ahead = [&](uint32_t a_, uint32_t b_, uint32_t by) { return WORD == RouteWord::kLogit16 || b_ <= kOutWord || a_ >= b_ + by; };
 
-    // ---- groups: whole lanes, 2^i of them, have one
+    // ---- groups
     if (a.groups > 1u) {
-        const uint32_t lanes = a.group_size / NPL, group = sub / lanes;
+        const uint32_t lanes = 1u << a.group_shift;
         uint32_t best = 0, second = 0;
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
@@ -374,6 +377,7 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
         if (lanes >= 4u) merge(dpp_keep_u32<0x4E>(best), dpp_keep_u32<0x4E>(second));
         if (lanes >= 8u) merge(dpp_keep_u32<0x141>(best), dpp_keep_u32<0x141>(second));
         if (lanes >= 16u) merge(dpp_keep_u32<0x140>(best), dpp_keep_u32<0x140>(second));
+        if (lanes >= 32u) merge(__shfl_xor(best, 16), __shfl_xor(second, 16));
         uint32_t mark = best, by = apart;
         bool known = true;
         if (WORD != RouteWord::kLogit16 && a.group_top == 2u && best > kOutWord) {
@@ -382,7 +386,7 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
             by = 2u * apart;
         }
         if (WORD != RouteWord::kLogit16) known &= best != 2u;
-        const bool counts = sub * NPL < a.experts;
+        const bool counts = group < a.groups;
         uint32_t word = counts ? (mark + 1u) << 6 | (63u - group) : 0u, last = 0;
         bool kept = false;
         for (uint32_t r = 0; r < a.kept; ++r) {
@@ -529,41 +533,45 @@ static void launch_route_fast(const RouteArgs &a, hipStream_t s) {
     else if (a.logits_type == SHRIKE_ELEM_F32) hipLaunchKernelGGL((k_route_rows_fast<LANES, NPL, RouteWord::kLogit>), dim3(blocks), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((k_route_rows_fast<LANES, NPL, RouteWord::kLogit16>), dim3(blocks), dim3(256), 0, s, a);
 }
-// the experts a lane for a row of 2^i lanes
-static uint32_t experts_a_lane(uint32_t experts, uint32_t lanes) {
-    uint32_t n = 1;
-    while (n * lanes < experts) n *= 2u;
-    return n;
-}
 constexpr uint32_t kRowsForNarrow = 2048;
-// Whether groups are 2^i whole lanes, up to 16.
-static bool groups_are_lanes(const RouteArgs &a, uint32_t per_lane) {
-    if (a.groups == 1u) return true;
-    const uint32_t lanes = a.group_size / per_lane;
-    return a.group_size % per_lane == 0 && lanes <= 16u && (lanes & (lanes - 1u)) == 0;
+// How a row's experts lie in `lanes` lanes: 2^shift lanes a group (of one group: all), `each` experts a lane, also 2^i. each > 32: they do not.
+struct RouteLanes {
+    uint32_t shift = 0, each = 64;
+};
+static RouteLanes lanes_of(const RouteArgs &a, uint32_t lanes) {
+    RouteLanes l;
+    uint32_t groups = 1;
+    while (groups < a.groups) groups *= 2u;
+    if (groups > lanes) return l;
+    while ((lanes / groups) >> (l.shift + 1u)) ++l.shift;
+    l.each = 1;
+    while ((l.each << l.shift) < a.group_size) l.each *= 2u;
+    return l;
 }
 
-static void launch_route(const RouteArgs &a, hipStream_t s) {
-    const uint32_t wide = experts_a_lane(a.experts, 64), narrow = experts_a_lane(a.experts, 16);
-    if (a.rows >= kRowsForNarrow && narrow <= 32u && groups_are_lanes(a, narrow)) {
-        if (narrow <= 1u) launch_route_fast<16, 1>(a, s);
-        else if (narrow == 2u) launch_route_fast<16, 2>(a, s);
-        else if (narrow == 4u) launch_route_fast<16, 4>(a, s);
-        else if (narrow == 8u) launch_route_fast<16, 8>(a, s);
-        else if (narrow == 16u) launch_route_fast<16, 16>(a, s);
+static void launch_route(RouteArgs a, hipStream_t s) {
+    const RouteLanes narrow = lanes_of(a, 16), wide = lanes_of(a, 64);
+    if (a.rows >= kRowsForNarrow && narrow.each <= 32u) {
+        a.group_shift = narrow.shift;
+        if (narrow.each == 1u) launch_route_fast<16, 1>(a, s);
+        else if (narrow.each == 2u) launch_route_fast<16, 2>(a, s);
+        else if (narrow.each == 4u) launch_route_fast<16, 4>(a, s);
+        else if (narrow.each == 8u) launch_route_fast<16, 8>(a, s);
+        else if (narrow.each == 16u) launch_route_fast<16, 16>(a, s);
         else launch_route_fast<16, 32>(a, s);
-    } else if (groups_are_lanes(a, wide)) {
-        if (wide <= 1u) launch_route_fast<64, 1>(a, s);
-        else if (wide == 2u) launch_route_fast<64, 2>(a, s);
-        else if (wide == 4u) launch_route_fast<64, 4>(a, s);
-        else if (wide == 8u) launch_route_fast<64, 8>(a, s);
+    } else if (wide.each <= 16u) {
+        a.group_shift = wide.shift;
+        if (wide.each == 1u) launch_route_fast<64, 1>(a, s);
+        else if (wide.each == 2u) launch_route_fast<64, 2>(a, s);
+        else if (wide.each == 4u) launch_route_fast<64, 4>(a, s);
+        else if (wide.each == 8u) launch_route_fast<64, 8>(a, s);
         else launch_route_fast<64, 16>(a, s);
     } else {
         const dim3 blocks(std::min((a.rows - 1u) / 4u + 1u, 65536u)), threads(256);
-        if (wide <= 1u) hipLaunchKernelGGL((k_route_rows<1>), blocks, threads, 0, s, a);
-        else if (wide == 2u) hipLaunchKernelGGL((k_route_rows<2>), blocks, threads, 0, s, a);
-        else if (wide == 4u) hipLaunchKernelGGL((k_route_rows<4>), blocks, threads, 0, s, a);
-        else if (wide == 8u) hipLaunchKernelGGL((k_route_rows<8>), blocks, threads, 0, s, a);
+        if (a.experts <= 64u) hipLaunchKernelGGL((k_route_rows<1>), blocks, threads, 0, s, a);
+        else if (a.experts <= 128u) hipLaunchKernelGGL((k_route_rows<2>), blocks, threads, 0, s, a);
+        else if (a.experts <= 256u) hipLaunchKernelGGL((k_route_rows<4>), blocks, threads, 0, s, a);
+        else if (a.experts <= 512u) hipLaunchKernelGGL((k_route_rows<8>), blocks, threads, 0, s, a);
         else hipLaunchKernelGGL((k_route_rows<16>), blocks, threads, 0, s, a);
     }
 }
@@ -608,7 +616,7 @@ extern "C" int shrike_hip_route_rows(void *stream, const shrike_route_desc *desc
     a.top_k = desc->top_k;
     a.groups = desc->kept_groups == desc->groups ? 1u : desc->groups;  // all of them kept: as if there were none
     a.kept = desc->kept_groups;
-    a.group_size = size;
+    a.group_size = a.groups == 1u ? a.experts : size;
     a.logits_type = logits_dtype;
     a.bias_type = bias_dtype;
     a.weights_type = weights_dtype;
@@ -617,8 +625,8 @@ extern "C" int shrike_hip_route_rows(void *stream, const shrike_route_desc *desc
     a.renormalize = desc->renormalize != 0;
     a.scaling = desc->scaling;
     const uint64_t size_of = logits_dtype == SHRIKE_ELEM_F32 ? 4u : 2u;
-    a.whole = reinterpret_cast<uintptr_t>(d_logits) % 16u == 0 && (rows == 1u || logits_stride_elements * size_of % 16u == 0) && a.experts * size_of % 16u == 0;
-    a.whole_bias = d_bias && reinterpret_cast<uintptr_t>(d_bias) % 16u == 0 && a.experts * (bias_dtype == SHRIKE_ELEM_F32 ? 4u : 2u) % 16u == 0;
+    a.whole = reinterpret_cast<uintptr_t>(d_logits) % 16u == 0 && (rows == 1u || logits_stride_elements * size_of % 16u == 0) && a.group_size * size_of % 16u == 0;
+    a.whole_bias = d_bias && reinterpret_cast<uintptr_t>(d_bias) % 16u == 0 && a.group_size * (bias_dtype == SHRIKE_ELEM_F32 ? 4u : 2u) % 16u == 0;
     constexpr uint32_t kMostRows = 1u << 24;  // of a launch, which holds fewer than 2^32 threads
     for (uint32_t done = 0; done < rows; done += kMostRows) {
         RouteArgs part = a;

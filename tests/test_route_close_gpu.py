@@ -100,3 +100,24 @@ def test_where_one_form_gives_way_to_the_next(gpu, rows, experts, groups, kept):
         i2, b2 = call(d, logits[order], None, logits_type=kind)
         assert np.array_equal(i2, want[0][order])
         ref.assert_weights(b2, want[1][order], want[2][order], capi.ELEM_F16)
+
+
+@pytest.mark.parametrize("experts,groups,kept,top_k", [(100, 4, 2, 32), (72, 8, 4, 32), (912, 8, 4, 32), (344, 4, 3, 16), (96, 3, 2, 8), (96, 3, 1, 32), (60, 6, 2, 5), (1024, 64, 9, 20),
+                                                       (512, 2, 1, 10), (1000, 2, 1, 16), (999, 3, 2, 8), (1023, 33, 5, 32), (992, 62, 7, 16), (77, 7, 3, 8), (650, 26, 4, 8), (30, 15, 4, 6),
+                                                       (64, 64, 8, 8), (1024, 2, 1, 32), (510, 17, 3, 9), (144, 9, 2, 8), (128, 2, 1, 8), (20, 5, 2, 3), (3, 3, 2, 2), (48, 16, 3, 9),
+                                                       (800, 32, 4, 30)])
+def test_groups_of_any_size(gpu, experts, groups, kept, top_k):
+    r = np.random.default_rng(experts + groups)
+    for scores, best, kind, biased in ((SIGMOID, 2, F32, True), (SOFTMAX, 1, capi.ELEM_BF16, False), (SOFTMAX, 2, capi.ELEM_F16, True), (SIGMOID, 1, F32, False)):
+        logits = r.normal(0, 1.5, (53, experts))
+        logits[40:, r.permutation(experts)[:experts // 4]] = -np.inf
+        logits[45:48, :experts // groups] = np.nan
+        logits = ref.decode(ref.encode(logits, kind), kind)
+        bias = r.normal(0, 0.05, experts).astype(np.float32).astype(np.float64) if biased else None
+        d = ref.desc(experts, top_k, scores, groups, kept, best)
+        want = ref.route(d, logits, bias)
+        for rows, pad in ((1, 0), (53, 8), (2050, 3)):
+            order = np.arange(rows) % 53
+            i2, b2 = call(d, logits[order], bias, logits_type=kind, weights_type=F32, pad=pad)
+            assert np.array_equal(i2, want[0][order]), f"{rows} rows"
+            ref.assert_weights(b2, want[1][order], want[2][order], F32, f"{rows} rows")
