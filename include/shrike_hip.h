@@ -657,8 +657,10 @@ int shrike_hip_route_rows(void *stream, const shrike_route_desc *desc, const voi
  * w->weights: codes u8[n, k / 2], 16-byte aligned; scales and biases: 16-bit [n, k / group_size] of meta_dtype, all without gaps. group_size: 32,
  * 64 (this library's own) or 128; k: a multiple of group_size up to SHRIKE_AFFINE4_MAX_K; n up to 2^24; rows up to 2^22. x: fp16 or bf16, rows at 16-byte
  * aligned addresses, x_stride_elements apart (at most 2^36); out: fp16, bf16 or fp32, rows out_stride_elements apart (what lies between them is left as it
- * is). The codes are never rounded: products of a group are summed and scaled in fp32 and the result is rounded once. The order of these sums
- * depends on rows, n and k, so calls of other sizes may differ in last places; the same call gives the same bits. */
+ * is). The codes are never rounded: products of a group are summed and scaled in fp32 and the result is rounded once. A group's sums of x * code (up
+ * to 15 a value) and of x have to be finite in fp32; a row of x with an infinity or a NaN has outputs that are not finite, and no other row's change. The
+ * order of the sums depends on rows, n and k, so calls of other sizes may differ in last places; the same call gives the same bits. out overlaps
+ * no input. */
 int shrike_hip_affine4_product(void *stream, const void *d_x, uint32_t x_dtype, uint64_t x_stride_elements, const shrike_projection *w,
                                uint32_t meta_dtype, uint32_t group_size, const void *d_bias, void *d_out, uint32_t out_dtype,
                                uint64_t out_stride_elements, uint32_t rows, uint32_t n, uint32_t k);

@@ -106,6 +106,8 @@ __device__ __forceinline__ void affine4_store(const Affine4Args &a, uint32_t r, 
 // A matrix-vector product is the reading of its weights. Lanes side by side read a row's 16-byte chunks (32 codes) side by side: 2^shift lanes a
 // row, NCH chunks each, so that rows of any length leave few lanes idle (90 chunks of 2,880 k are three steps of 32 lanes, 94 %). A wave holds its
 // slices of x in registers and takes a batch of rows a turn, turn after turn. (A row of x too long for that is read piece by piece with every turn.)
+// The memory bounds it: 201,088 x 2,880 takes 65 us, 5.0 TB/s of all its bytes; 65,536 x 8,192 63 us, 4.7 TB/s. (A lane a row with x in LDS took 123 us of
+// the first.) A small one is its launch: 2,048 x 2,048 3.8 us on the GPU.
 constexpr int kGemvChunks = 6;
 template <int NCH>
 constexpr int kGemvBatch = NCH <= 2 ? 4 : 2;  // rows a lane and turn: eight to twelve loads on their way
@@ -566,10 +568,17 @@ static int launch_few(const Affine4Args &args, hipStream_t s) {
 }
 // ------------------------------------------------------------------ many rows
 //
-// 32 MT WM rows against 32 NT WN outputs a workgroup of WM x WN waves, 32 MT x 32 NT a wave. Rows and codes come through LDS, a step of 64 k of the rows
-// two steps ahead in three places, two steps of the codes (64 bytes a row) in two. A chunk is eight chains (a chain is a group's products, or
-// half a group's of 128): its scales are a lane's own loads, a chunk ahead, and the bias term is added a chunk behind from the sums of the rows' groups,
-// which the waves form from the operands that they hold, WN waves a share of the tile's rows each.
+// 32 MT WM rows against 32 NT WN outputs a workgroup of KS parts of WM x WN waves, 32 MT x 32 NT a wave; the parts have a share of k each and their sums meet
+// in LDS. Rows and codes come through LDS, a step of 64 k of the rows two steps ahead in three places, two steps of the codes (64 bytes a row) in two. A
+// chunk is eight chains (a chain is a group's products, or half a group's of 128): its scales and biases come through LDS too, a chunk ahead, and the
+// bias term is added a chunk behind from the sums of the rows' groups, which the waves form from the operands that they hold, WN waves a share of the
+// tile's rows each. A wave takes a code apart for MT blocks of rows, and scales a chain while the next is multiplied.
+//
+// What bounds it is the issue of instructions beside the matrix ones: a step of a wave of 128 x 64 has 32 of these, 1,024 cycles, and some 390 of the vector
+// unit, half of them the scaling. 4,096 rows of 8,192 x 4,096: 326 us, 840 TFLOP/s (a large fp16 product of the library, whose weights are not taken
+// apart, 227); 512 of 8,192 x 2,048: 34 us. Without the loads the large one takes 12 % less, without the group sums 10 to 15. In two parts of k a CU
+// with one small tile has two waves a SIMD: 512 of 8,192 x 2,048 39 us against 44.
+
 // Four bytes a lane into LDS, as lds_load16
 __device__ __forceinline__ void lds_load4(uint32_t lds, const void *base, uint32_t offset) {
     const void *moved;

@@ -182,11 +182,14 @@ __global__ __launch_bounds__(256) void k_route_rows(RouteArgs a) {
 // 64 bits are needed where two choices lie close together, and that is seldom: here a choice is a 32-bit word, its value in fixed point below the row's
 // largest (22 bits) over the expert's number (10, so that the lower one is the larger word), from fp32 arithmetic whose error is under two
 // units. The words' order is the choices' order where neighbours in it, the last one taken and the first one left among them, are as far
-// apart as both may be off; a row where they are not is routed again by route_row. Where the logits
-// themselves decide and have 16 bits, the word is all of them over the number, and exact.
+// apart as both may be off. Where some of them are not, the words next in order are taken too, up to a gap, and the scores of those alone are formed and
+// put into order in 64 bits; a row without a gap in 32, or whose groups lie too close, is routed again by route_row. Where the logits themselves
+// decide and have 16 bits, the word is all of them over the number, and exact.
 //
-// LANES lanes have a row, each NPL neighbouring experts: 64 for few rows, which takes the fewest steps, 16 for many, where four rows share every step
-// between lanes. A step of the selection is the largest of a lane's words below the last one taken, and then of the row's lanes.
+// LANES lanes have a row, each up to NPL neighbouring experts of one group: 64 for few rows, which takes the fewest steps, 16 for many, where four rows
+// share every step between lanes. A step of the selection is the largest of a lane's words below the last one taken, and then of the row's lanes. The vector unit bounds it: 16,384 rows of 512, top 10, take 20 to 22 us where
+// their bytes take 7 (in 64 bits alone 75; every close row again in 64 bits 33; words with a test of range each 30). One row takes 3.2 us on the GPU, and
+// a call from the host 8.
 
 enum class RouteWord { kValue, kLogit, kLogit16 };
 constexpr float kUnits = 4194296.0f;  // 2^22 - 8
@@ -533,7 +536,9 @@ static void launch_route_fast(const RouteArgs &a, hipStream_t s) {
     else if (a.logits_type == SHRIKE_ELEM_F32) hipLaunchKernelGGL((k_route_rows_fast<LANES, NPL, RouteWord::kLogit>), dim3(blocks), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((k_route_rows_fast<LANES, NPL, RouteWord::kLogit16>), dim3(blocks), dim3(256), 0, s, a);
 }
-constexpr uint32_t kRowsForNarrow = 2048;
+// 16 lanes a row against 64: 2,048 rows of 512 11 us against 7.5, 8,192 16.6 against 15.8 (of 256 in groups 12.0 against 12.8, of 64 6.5 against 7.0),
+// 16,384 22 against 27 (18 against 22, 7.7 against 10.8).
+constexpr uint32_t kRowsForNarrow = 8192;
 // How a row's experts lie in `lanes` lanes: 2^shift lanes a group (of one group: all), `each` experts a lane, also 2^i. each > 32: they do not.
 struct RouteLanes {
     uint32_t shift = 0, each = 64;

@@ -34,7 +34,7 @@ def test_close_choices(gpu, experts, top_k, scores, biased):
     for renormalize in (True, False):
         d = ref.desc(experts, top_k, scores, renormalize=renormalize)
         got, bits = check(d, logits, bias, weights_type=F32, what=f"{experts}")
-        order = r.permutation(np.arange(4096) % len(logits))  # the same rows among others, where there are many
+        order = r.permutation(np.arange(9001) % len(logits))  # the same rows among others, where there are many
         i2, b2 = call(d, logits[order], bias, weights_type=F32)
         want = ref.route(d, logits, bias)
         assert np.array_equal(i2, want[0][order]), f"{experts}: {np.argwhere((i2 != want[0][order]).any(1))[:4].ravel()}"
@@ -56,7 +56,7 @@ def test_close_groups(gpu, experts, top_k, groups, kept, scores, best):
     for bias in (None, r.integers(-3, 4, experts) * 2.0 ** -20):
         d = ref.desc(experts, top_k, scores, groups, kept, best)
         check(d, logits, bias, weights_type=F32)
-        order = r.permutation(np.arange(4096) % len(logits))
+        order = r.permutation(np.arange(9001) % len(logits))
         i2, b2 = call(d, logits[order], bias, weights_type=F32)
         want = ref.route(d, logits, bias)
         assert np.array_equal(i2, want[0][order])
@@ -81,13 +81,13 @@ def test_far_and_odd_values_in_many_rows(gpu, experts, top_k):
         for renormalize in (True, False):
             d = ref.desc(experts, top_k, scores, renormalize=renormalize)
             want = ref.route(d, logits, b)
-            order = r.permutation(np.arange(4096) % len(logits))
+            order = r.permutation(np.arange(9001) % len(logits))
             i2, b2 = call(d, logits[order], b, weights_type=F32)
             assert np.array_equal(i2, want[0][order])
             ref.assert_weights(b2, want[1][order], want[2][order], F32)
 
 
-@pytest.mark.parametrize("rows", [2047, 2048, 2049, 2050, 2051])
+@pytest.mark.parametrize("rows", [8191, 8192, 8193, 8194, 8195])
 @pytest.mark.parametrize("experts,groups,kept", [(64, 1, 1), (512, 1, 1), (256, 8, 4), (320, 1, 1)])
 def test_where_one_form_gives_way_to_the_next(gpu, rows, experts, groups, kept):
     r = np.random.default_rng(rows)
@@ -116,7 +116,7 @@ def test_groups_of_any_size(gpu, experts, groups, kept, top_k):
         bias = r.normal(0, 0.05, experts).astype(np.float32).astype(np.float64) if biased else None
         d = ref.desc(experts, top_k, scores, groups, kept, best)
         want = ref.route(d, logits, bias)
-        for rows, pad in ((1, 0), (53, 8), (2050, 3)):
+        for rows, pad in ((1, 0), (53, 8), (8194, 3)):
             order = np.arange(rows) % 53
             i2, b2 = call(d, logits[order], bias, logits_type=kind, weights_type=F32, pad=pad)
             assert np.array_equal(i2, want[0][order]), f"{rows} rows"
