@@ -1120,7 +1120,7 @@ extern "C" int shrike_hip_affine4_product(void *stream, const void *d_x, uint32_
     a.group = group_size;
     a.meta = meta_dtype;
     a.out_type = out_dtype;
-    constexpr uint32_t kMost = 16u * 65535u;  // rows of a launch: a grid's second dimension ends at 65,535
+    constexpr uint32_t kMost = 8u * 65535u;  // rows of a launch: a grid's second dimension ends at 65,535, and the lowest workgroup has 8 rows
     for (uint32_t first = 0; first < rows; first += kMost) {
         Affine4Args part = a;
         part.x += uint64_t(first) * a.x_stride;

@@ -114,3 +114,35 @@ def test_weights_used_by_calls_at_once_and_again(gpu, rows):
             bits = out.download(np.uint16, rows * n)
             first = bits if first is None else first
             assert np.array_equal(bits, first)
+
+
+@pytest.mark.parametrize("rows", [8 * 65535 - 1, 8 * 65535, 8 * 65535 + 1, 8 * 65535 + 70, 1 << 20, 1 << 22])
+def test_more_rows_than_a_launch_takes(gpu, rows):
+    """Whole rows of a few kinds, over and over; every row of the output by its kind."""
+    r = np.random.default_rng(rows % 1000)
+    n, k, kinds = 24, 64, 61
+    w = ref.Weights(r, n, k, whole=True)
+    x = ref.whole_rows(r, kinds, k, F16)
+    want = ref.encode(ref.decode(x, F16) @ w.values.T, F32)
+    which = np.arange(rows) % kinds
+    got = ref.run(x[which], F16, w, None, F32)
+    assert np.array_equal(got, want[which])
+
+
+@pytest.mark.parametrize("rows", [1, 3, 20, 70])
+@pytest.mark.parametrize("group", [32, 64])
+def test_as_many_outputs_as_there_may_be(gpu, rows, group):
+    r = np.random.default_rng(rows)
+    n, k, piece = 1 << 24, group, 4096
+    w = ref.Weights(r, piece, k, group, whole=True)
+    x = ref.whole_rows(r, rows, k, F16)
+    want = ref.encode(ref.decode(x, F16) @ w.values.T, F32)
+    times = n // piece
+    codes, scales, biases = (rt.dev(np.tile(v, (times, 1))) for v in (w.codes, w.scale_bits, w.bias_bits))
+    out = rt.DeviceBuffer(rows * n * 4)
+    dx = rt.dev(x)
+    rt.affine4_product(dx, F16, k, codes, scales, biases, w.meta, group, None, out, F32, n, rows, n, k)
+    rt.synchronize()
+    for i in {0, rows // 2, rows - 1}:
+        got = out.download(np.float32, n, i * n * 4).reshape(times, piece)
+        assert np.array_equal(got, np.broadcast_to(want[i], got.shape)), i

@@ -3,7 +3,7 @@ is put in order at once, near ties across the end of the route and between group
 import numpy as np
 import pytest
 
-from shrike_amd import capi
+from shrike_amd import capi, runtime as rt
 from tests import route_reference as ref
 from tests.test_route_rows_gpu import F32, SIGMOID, SOFTMAX, call, check
 
@@ -121,3 +121,23 @@ def test_groups_of_any_size(gpu, experts, groups, kept, top_k):
             i2, b2 = call(d, logits[order], bias, logits_type=kind, weights_type=F32, pad=pad)
             assert np.array_equal(i2, want[0][order]), f"{rows} rows"
             ref.assert_weights(b2, want[1][order], want[2][order], F32, f"{rows} rows")
+
+
+@pytest.mark.parametrize("rows", [(1 << 24) - 1, 1 << 24, (1 << 24) + 5, 40_000_000])
+def test_more_rows_than_a_launch_takes(gpu, rows):
+    r = np.random.default_rng(rows % 1000)
+    experts, kinds = 4, 1009
+    logits = r.normal(0, 1.5, (kinds, experts))
+    bits = ref.encode(logits, capi.ELEM_F16)
+    d = ref.desc(experts, 1, SIGMOID, renormalize=False)
+    want, weights, bound = ref.route(d, ref.decode(bits, capi.ELEM_F16))
+    x = rt.dev(np.tile(bits, (rows // kinds + 1, 1))[:rows])
+    idx, w = rt.empty(rows * 4 + 64).fill(0xA5), rt.empty(rows * 4 + 64).fill(0xA5)
+    rt.route_rows(d, x, capi.ELEM_F16, experts, None, F32, idx, w, F32, rows)
+    rt.synchronize()
+    which = np.arange(rows) % kinds
+    assert np.array_equal(idx.download(np.uint32, rows), want[which, 0])
+    got = w.download(np.float32, rows)
+    assert np.array_equal(got, got[:kinds][which])  # (a row's route depends on that row alone)
+    ref.assert_weights(got[:kinds, None], weights, bound, F32)
+    assert np.all(idx.download(np.uint8, 64, rows * 4) == 0xA5) and np.all(w.download(np.uint8, 64, rows * 4) == 0xA5)
