@@ -812,7 +812,10 @@ __global__ __launch_bounds__(64 * WM * WN * KS, 2) void k_affine4_tile(Affine4Ar
 #pragma unroll
         for (int c = 0; c < kSubs; ++c)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) factors[c][i] = meta_f32(next_scales[c][i], a.meta);
+            for (int i = 0; i < NT; ++i) {
+                // (past the row's end there is no second group, but the next output's first scale, which may be anything)
+                factors[c][i] = SUB32 && c == 1 && 64u * g + 32u >= my_k ? 0.0f : meta_f32(next_scales[c][i], a.meta);
+            }
         auto slots = [&](auto slot_) {  // an instruction and what stands behind it
             constexpr int slot = decltype(slot_)::value, j = slot % kPer, chain = slot / kPer, i = chain % NT, c = chain / NT % kSubs, m = chain / NT / kSubs;
             constexpr int chains = MT * kSubs * NT, last = (chain + chains - 1) % chains, at = c * kPer + j;

@@ -22,7 +22,7 @@ def test_edges(gpu, rows, n, k, group):
     exactly(r, rows, n, k, group, F16 if k % 3 else BF16, F32, meta=F16 if group == 32 else BF16, symmetric=k == 64, bias=k == 128)
 
 
-@pytest.mark.parametrize("rows,n", [(1700, 1900), (1800, 7200)])
+@pytest.mark.parametrize("rows,n", [(25473, 70), (1700, 1900), (1800, 7200)])
 @pytest.mark.parametrize("k,group", [(64, 32), (96, 32), (128, 64), (160, 32), (192, 64), (256, 32), (320, 64), (384, 128), (448, 64), (480, 32), (512, 128), (544, 32), (576, 64), (640, 128),
                                      (1024, 64), (1056, 32), (1088, 64), (1152, 128), (2304, 64)])
 def test_lengths(gpu, rows, n, k, group):
@@ -146,3 +146,20 @@ def test_as_many_outputs_as_there_may_be(gpu, rows, group):
     for i in {0, rows // 2, rows - 1}:
         got = out.download(np.float32, n, i * n * 4).reshape(times, piece)
         assert np.array_equal(got, np.broadcast_to(want[i], got.shape)), i
+
+
+@pytest.mark.parametrize("rows,n", [(1, 300), (5, 300), (20, 300), (64, 16384), (25473, 70), (3600, 3500)])
+@pytest.mark.parametrize("k", [32, 96, 160, 288])
+@pytest.mark.parametrize("value", [0x7FC0, 0x7F80])
+def test_scales_of_the_next_output_do_not_count(gpu, rows, n, k, value):
+    """Rows of an odd number of groups of 32: where the last one ends in the middle of a step, the next output's scales and biases stand behind."""
+    r = np.random.default_rng(k)
+    w = ref.Weights(r, n, k, 32, whole=True)
+    x = ref.whole_rows(r, rows, k, F16)
+    want = ref.decode(x, F16) @ w.values.T
+    bad = [1, 32, 64, n // 2, n - 1]
+    w.scale_bits[bad] = value
+    w.bias_bits[bad] = value
+    got = ref.run(x, F16, w, None, F32)
+    good = np.setdiff1d(np.arange(n), bad)
+    ref.assert_exact(np.ascontiguousarray(got[:, good]), want[:, good], F32)
