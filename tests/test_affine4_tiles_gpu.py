@@ -77,13 +77,14 @@ def test_rows_past_4_gib_in_tiles(gpu, rows, n):
         assert np.array_equal(far_out.download(np.float32, n, i * out_stride * 4), want[i]), i
 
 
-def test_nan_stays_in_its_row_and_output_of_large_tiles(gpu):
+@pytest.mark.parametrize("rows,n", [(3600, 3500), (25473, 70)])
+def test_nan_stays_in_its_row_and_output_of_tiles(gpu, rows, n):
     r = np.random.default_rng(5)
-    rows, n, k = 3600, 3500, 256
+    k = 256
     w = ref.Weights(r, n, k, whole=True)
     x = ref.whole_rows(r, rows, k, F16)
     want = ref.decode(x, F16) @ w.values.T
-    bad_rows, bad_outputs = [0, 255, 256, 1801, 3599], [0, 31, 32, 1777, 3499]
+    bad_rows, bad_outputs = [0, 255, 256, 1801, rows - 1], [0, 31, 32, n // 2 + 5, n - 1]
     for i, value in zip(bad_rows, (0x7E00, 0x7C00, 0xFC00, 0x7E00, 0x7C00)):
         x[i, (i * 7) % k] = value
     for i in bad_outputs:
@@ -163,3 +164,24 @@ def test_scales_of_the_next_output_do_not_count(gpu, rows, n, k, value):
     got = ref.run(x, F16, w, None, F32)
     good = np.setdiff1d(np.arange(n), bad)
     ref.assert_exact(np.ascontiguousarray(got[:, good]), want[:, good], F32)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 301), (4, 301), (20, 301), (64, 16384), (25473, 70), (3600, 3500)])
+@pytest.mark.parametrize("k,group", [(96, 32), (320, 64)])
+def test_scales_biases_and_outputs_at_addresses_of_their_own_size(gpu, rows, n, k, group):
+    r = np.random.default_rng(rows)
+    w = ref.Weights(r, n, k, group, F16, whole=True)
+    x, own = ref.whole_rows(r, rows, k, F16), ref.encode(r.integers(-9, 10, n) * 0.5, F16)
+    want = ref.encode(ref.decode(x, F16) @ w.values.T + ref.decode(own, F16), F16)
+
+    def behind(a, offset):  # the array `offset` bytes behind an allocation's start
+        buf = rt.empty(a.nbytes + 64)
+        buf.upload(np.ascontiguousarray(a).view(np.uint8).reshape(-1), offset)
+        return buf
+
+    dx, codes, scales, biases, bias = rt.dev(x), rt.dev(w.codes), behind(w.scale_bits, 2), behind(w.bias_bits, 6), behind(own, 10)
+    out = rt.empty(rows * n * 2 + 64).fill(0xA5)
+    rt.affine4_product(dx, F16, k, codes, scales.ptr + 2, biases.ptr + 6, w.meta, group, bias.ptr + 10, out.ptr + 14, F16, n, rows, n, k)
+    rt.synchronize()
+    assert np.array_equal(out.download(np.uint16, rows * n, 14).reshape(rows, n), want)
+    assert np.all(out.download(np.uint8, 14) == 0xA5) and np.all(out.download(np.uint8, 50, rows * n * 2 + 14) == 0xA5)
