@@ -381,12 +381,13 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
         if (lanes >= 8u) merge(dpp_keep_u32<0x141>(best), dpp_keep_u32<0x141>(second));
         if (lanes >= 16u) merge(dpp_keep_u32<0x140>(best), dpp_keep_u32<0x140>(second));
         if (lanes >= 32u) merge(__shfl_xor(best, 16), __shfl_xor(second, 16));
-        uint32_t mark = best, by = apart;
+        // (the same in every lane, also of groups out of service and past the last: the row is certain in all of its lanes or in none)
+        const uint32_t by = WORD != RouteWord::kLogit16 && a.group_top == 2u ? 2u * apart : apart;
+        uint32_t mark = best;
         bool known = true;
         if (WORD != RouteWord::kLogit16 && a.group_top == 2u && best > kOutWord) {
             known = second > 2u && best > 2u;  // (what is missing counts 0, and what lies too low is not known: both by route_row)
             mark = best + second;
-            by = 2u * apart;
         }
         if (WORD != RouteWord::kLogit16) known &= best != 2u;
         const bool counts = group < a.groups;
