@@ -18,6 +18,7 @@ struct RouteArgs {
     uint32_t logits_type, bias_type, weights_type, group_top, sigmoid, renormalize;
     float scaling;
     uint32_t group_shift;        // 2^i lanes have a group
+    float levels;                // of the additions of a row's experts in pairs
     uint32_t whole, whole_bias;  // rows (the bias) and their groups start at multiples of 16 bytes and are multiples of 16 bytes long
 };
 
@@ -180,8 +181,8 @@ __global__ __launch_bounds__(256) void k_route_rows(RouteArgs a) {
 // ------------------------------------------------------------------ many rows at once
 //
 // 64 bits are needed where two choices lie close together, and that is seldom: here a choice is a 32-bit word, its value in fixed point below the row's
-// largest (22 bits) over the expert's number (10, so that the lower one is the larger word), from fp32 arithmetic whose error is under two
-// units. The words' order is the choices' order where neighbours in it, the last one taken and the first one left among them, are as far
+// largest (22 bits) over the expert's number (10, so that the lower one is the larger word), from fp32 arithmetic whose error has a
+// bound. The words' order is the choices' order where neighbours in it, the last one taken and the first one left among them, are as far
 // apart as both may be off. Where some of them are not, the words next in order are taken too, up to a gap, and the scores of those alone are formed and
 // put into order in 64 bits; a row without a gap in 32, or whose groups lie too close, is routed again by route_row. Where the logits themselves
 // decide and have 16 bits, the word is all of them over the number, and exact.
@@ -193,6 +194,14 @@ __global__ __launch_bounds__(256) void k_route_rows(RouteArgs a) {
 
 enum class RouteWord { kValue, kLogit, kLogit16 };
 constexpr float kUnits = 4194296.0f;  // 2^22 - 8
+// How far a score in fp32 may be off, in 2^-24. exp_fast of -x: its argument has two or three roundings and the constant's, which count x times, and the
+// instruction 2 (one place), (2.25 x + 2) of it: for a softmax up to 2.1 of the largest term, which is 1. The softmax's sum, of 2^i experts: what its terms
+// are off, under i + 2 of the sum (11.7 where 1,023 of them lie near x = 5 beside the 1), its additions in pairs i, its reciprocal 2. That factor is one for the
+// whole row and moves a choice against another, as the bias is not scaled with it, by 2 i + 4 of the scores' difference. Two choices of a softmax: 2 * 2.1 + 2 i + 4
+// of the largest score at most; of sigmoids, s (1 - s) (1.25 x + 2) + 3 s each, under 3.2.
+__device__ __forceinline__ float softmax_off(float levels) { return (levels + 4.25f) * 0x1p-24f; }
+__device__ __forceinline__ float softmax_sum_off(float levels) { return (2.0f * levels + 5.0f) * 0x1p-24f; }
+constexpr float kSigmoidOff = 0x1p-22f;
 
 template <int LANES>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
@@ -302,13 +311,18 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     float inverse = 0.0f;  // of the softmax's sum, where it is wanted
     float v[NPL];
     if (!a.sigmoid && (WORD == RouteWord::kValue || !a.renormalize)) {
-        float total = 0.0f;
+        // (in pairs of neighbours, pairs of these, and so on: log2 of the experts' number roundings, where one after the other are as many as a lane has)
+        float part[6];  // part[i]: 2^i of them
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
             v[j] = exp_fast(l[j] - base);
-            total += v[j];
+            float sum = v[j];
+            int i = 0;
+#pragma unroll
+            for (; j >> i & 1; ++i) sum = part[i] + sum;
+            part[i] = sum;
         }
-        total = lanes_sum<LANES>(total);
+        const float total = lanes_sum<LANES>(part[__builtin_ctz(NPL)]);
         inverse = total > 0.0f ? __builtin_amdgcn_rcpf(total) : 0.0f;
     }
     auto score = [&](float v) { return a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + exp_fast(-v)) : exp_fast(v - base) * inverse; };
@@ -344,7 +358,7 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
             // all the row's choices, or as far down as 2; a choice is off by the score's few last places and by half a one of its own
             span = fminf(fmaxf(most + lanes_max<LANES>(-least), 0x1p-10f), 2.0f);
             certain = most == -INFINITY || fabsf(most) <= 4.0f;  // (further off, an fp32 is too coarse)
-            const float off = (a.sigmoid ? 1.0f : inverse) * 0x1p-22f + (fabsf(most) + span) * 0x1p-24f;
+            const float off = (a.sigmoid ? kSigmoidOff : inverse * softmax_off(a.levels)) + (fabsf(most) + span) * 0x1p-24f;
             apart = 3u + uint32_t(2.0f * off * (kUnits / span));
         }
         const float per_unit = kUnits / span, from = -(most - span) * per_unit;
@@ -429,7 +443,7 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     for (uint32_t i = 0; i < kSlots; ++i) place[i] = sub + i * LANES;
     if constexpr (WORD != RouteWord::kLogit16) {
         // Where words lie too close together, those that come next are taken too, up to a gap, and 64 bits put all that were taken into order: their
-        // scores alone, not the row's. (A softmax's sum stays the fp32 one: two choices whose difference it could turn are left to route_row.)
+        // scores alone, not the row's. (A softmax's sum stays the fp32 one: two choices whose difference it could turn, or hide, are left to route_row.)
         uint32_t left = largest_below(before), taken = a.top_k;
         auto gap = [&] { return left >= before || ahead(before >> kIndexBits, left >> kIndexBits, apart); };  // (not below: nothing is left)
         bool open = certain && !gap();
@@ -474,8 +488,8 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
 #pragma unroll
                     for (uint32_t i = 0; i < kSlots; ++i) {
                         rank[i] += v > mine[i] || (v == mine[i] && other < number[i]) ? 1u : 0u;
-                        if (!a.sigmoid && a.bias && sub + i * LANES < taken && v != mine[i] && v > -INFINITY && mine[i] > -INFINITY)
-                            known &= fabs(v - mine[i]) > fabs(of - my_score[i]) * 0x1p-20;
+                        if (!a.sigmoid && a.bias && sub + i * LANES < taken && of != my_score[i] && v > -INFINITY && mine[i] > -INFINITY)
+                            known &= fabs(v - mine[i]) > fabs(of - my_score[i]) * double(softmax_sum_off(a.levels));
                     }
             }
             __builtin_amdgcn_wave_barrier();
@@ -540,6 +554,11 @@ static void launch_route_fast(const RouteArgs &a, hipStream_t s) {
 // 16 lanes a row against 64: 2,048 rows of 512 11 us against 7.5, 8,192 16.6 against 15.8 (of 256 in groups 12.0 against 12.8, of 64 6.5 against 7.0),
 // 16,384 22 against 27 (18 against 22, 7.7 against 10.8).
 constexpr uint32_t kRowsForNarrow = 8192;
+static uint32_t levels_of(uint32_t n) {
+    uint32_t l = 0;
+    while ((1u << l) < n) ++l;
+    return l;
+}
 // How a row's experts lie in `lanes` lanes: 2^shift lanes a group (of one group: all), `each` experts a lane, also 2^i. each > 32: they do not.
 struct RouteLanes {
     uint32_t shift = 0, each = 64;
@@ -623,6 +642,7 @@ extern "C" int shrike_hip_route_rows(void *stream, const shrike_route_desc *desc
     a.groups = desc->kept_groups == desc->groups ? 1u : desc->groups;  // all of them kept: as if there were none
     a.kept = desc->kept_groups;
     a.group_size = a.groups == 1u ? a.experts : size;
+    a.levels = float(levels_of(a.groups) + levels_of(a.group_size));
     a.logits_type = logits_dtype;
     a.bias_type = bias_dtype;
     a.weights_type = weights_dtype;

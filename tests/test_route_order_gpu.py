@@ -74,3 +74,53 @@ def test_close_groups_beside_one_out_of_service(gpu, groups, size, top_k, scores
             by_bias[gone * size:(gone + 1) * size] = -np.inf
             for rows in (128, 9001):
                 compare(d, there, by_bias, rows, f"group {gone} is gone by its bias")
+
+
+def dominant_rows(experts, lanes):
+    """Rows of one expert with nearly all of the softmax and others of 0.97 * 2^-24 of it, where the additions of a sum in order, of a lane's sum in order and
+    of a sum in pairs each round them away; the rest is nothing."""
+    each, rows = experts // lanes, []
+    for small in ([*range(1, each), *(each << j for j in range(10))], [1 << j for j in range(10)], [*range(1, 20)], [*range(1, experts, 37)]):
+        row = np.full(experts, -100.0)
+        row[0] = 0.0
+        row[[e for e in small if e < experts - 1]] = np.log(0.97 * 2.0 ** -24)
+        rows.append(row)
+    return rows
+
+
+@pytest.mark.parametrize("experts", [64, 256, 512, 1024])
+@pytest.mark.parametrize("groups,best", [(1, 1), (8, 1), (8, 2)])
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_a_bias_that_cancels_a_dominant_expert(gpu, experts, groups, best, renormalize):
+    """What a softmax's sum in fp32 has lost does not move the choices: 64 bits decide between an expert of nearly 1 and a bias of nearly -1, and an expert of
+    nothing without a bias."""
+    logits = single(np.array(dominant_rows(experts, 64 if experts > 64 else 16) + dominant_rows(experts, 16)))
+    d = ref.desc(experts, 1, SOFTMAX, groups, 1, best, renormalize)
+    for m in range(-4, 21, 2):
+        bias = np.full(experts, -5e-4)
+        bias[0], bias[-1] = -1.0 + m * 2.0 ** -24, 0.0
+        if best == 2:  # the groups' second experts alike
+            bias[1], bias[-2] = -5e-4, -5e-4
+        bias = single(bias)
+        for rows in (len(logits), 8200):
+            compare(d, logits, bias, rows, f"{m} last places")
+
+
+@pytest.mark.parametrize("experts", [100, 512, 1000, 1024])
+@pytest.mark.parametrize("groups,best", [(1, 1), (4, 1), (4, 2)])
+def test_one_expert_above_many_equal_ones(gpu, experts, groups, best):
+    """One logit above equal ones, each of whose additions rounds the same way, and a bias that lifts one of these to the top one's choice or nearly."""
+    r = np.random.default_rng(experts + best)
+    d = ref.desc(experts, 1, SOFTMAX, groups, 1, best, False)
+    other = experts // max(groups, 2) + 5
+    for x in single(r.uniform(4.0, 10.0, 10)):
+        row = np.full(experts, -x)
+        row[0] = 0.0
+        p = np.exp(row) / np.exp(row).sum()
+        bias = np.zeros(experts)
+        bias[other] = p[0] - p[other]
+        bias = single(bias)
+        rows = np.tile(row, (48, 1))
+        rows[:, other] += np.append(0.0, r.choice([-1.0, 1.0], 47) * 2.0 ** r.uniform(-24, -17, 47)) / p[other]
+        for count in (48, 8200):
+            compare(d, single(rows), bias, count, f"{x} above the others")
