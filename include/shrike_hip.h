@@ -647,7 +647,7 @@ typedef struct {
 /* Routes of `rows` rows of logits (fp32, fp16 or bf16, SHRIKE_ELEM_*), logits_stride_elements apart, any address of their own size; d_bias:
  * [num_experts] of bias_dtype, or NULL. out_indices: u32[rows, top_k]; out_weights: [rows, top_k] of weights_dtype. They feed
  * shrike_hip_group_pairs and shrike_hip_moe_resolve_batch as the routers' outputs do (fp16 weights). `desc` is read at the call. A row's routes
- * depend on that row alone. */
+ * depend on that row alone: indices and weights are the same bits whatever the other rows and their number. */
 int shrike_hip_route_rows(void *stream, const shrike_route_desc *desc, const void *d_logits, uint32_t logits_dtype, uint64_t logits_stride_elements,
                           const void *d_bias, uint32_t bias_dtype, uint32_t *d_out_indices, void *d_out_weights, uint32_t weights_dtype,
                           uint32_t rows);

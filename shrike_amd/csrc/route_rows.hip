@@ -187,6 +187,9 @@ __global__ __launch_bounds__(256) void k_route_rows(RouteArgs a) {
 // put into order in 64 bits; a row without a gap in 32, or whose groups lie too close, is routed again by route_row. Where the logits themselves
 // decide and have 16 bits, the word is all of them over the number, and exact.
 //
+// Both sums, of all scores and of the chosen ones, are formed in pairs of neighbours, pairs of these and so on, an order that does not depend on the lanes
+// a row has: its weights are the same bits in a call of any size.
+//
 // LANES lanes have a row, each up to NPL neighbouring experts of one group: 64 for few rows, which takes the fewest steps, 16 for many, where four rows
 // share every step between lanes. A step of the selection is the largest of a lane's words below the last one taken, and then of the row's lanes. The vector unit bounds it: 16,384 rows of 512, top 10, take 20 to 22 us where
 // their bytes take 7 (in 64 bits alone 75; every close row again in 64 bits 33; words with a test of range each 30). One row takes 3.2 us on the GPU, and
@@ -503,7 +506,7 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
 
     // ---- the weights
     uint32_t index[kSlots];
-    float w[kSlots], most = -INFINITY, sum = 0.0f;
+    float w[kSlots], most = -INFINITY;
     bool served[kSlots];
 #pragma unroll
     for (uint32_t i = 0; i < kSlots; ++i) {
@@ -516,12 +519,11 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
     const bool among = a.renormalize && !a.sigmoid;  // the softmax of the chosen ones
     most = among ? lanes_max<LANES>(most) : 0.0f;
 #pragma unroll
-    for (uint32_t i = 0; i < kSlots; ++i) {
-        w[i] = !served[i] ? 0.0f : among ? exp_fast(w[i] - most) : score(w[i]);
-        sum += w[i];
-    }
+    for (uint32_t i = 0; i < kSlots; ++i) w[i] = !served[i] ? 0.0f : among ? exp_fast(w[i] - most) : score(w[i]);
     if (a.renormalize) {
-        sum = lanes_sum<LANES>(sum);
+        // (in the same order whatever the lanes: of neighbours, of pairs of these, and so on)
+        float sum = lanes_sum<LANES>(w[0]);
+        if constexpr (kSlots == 2) sum += lanes_sum<LANES>(w[1]);
         // (scores that fp32 does not hold well are 64 bits' again; none in service leaves zeros)
         if (a.sigmoid) certain &= sum > 1e-30f || lanes_max<LANES>(served[0] || served[kSlots - 1] ? 1u : 0u) == 0u;
         const float factor = sum > 0.0f ? a.scaling / sum : 0.0f;

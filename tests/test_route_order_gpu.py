@@ -124,3 +124,27 @@ def test_one_expert_above_many_equal_ones(gpu, experts, groups, best):
         rows[:, other] += np.append(0.0, r.choice([-1.0, 1.0], 47) * 2.0 ** r.uniform(-24, -17, 47)) / p[other]
         for count in (48, 8200):
             compare(d, single(rows), bias, count, f"{x} above the others")
+
+
+@pytest.mark.parametrize("experts,top_k,groups,kept", [(5, 3, 1, 1), (60, 8, 1, 1), (128, 32, 1, 1), (256, 8, 8, 4), (300, 20, 1, 1), (512, 10, 1, 1), (512, 32, 1, 1), (480, 24, 15, 4),
+                                                       (100, 17, 4, 2), (1000, 32, 1, 1)])
+@pytest.mark.parametrize("scores", [SOFTMAX, SIGMOID])
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("biased", [False, True])
+def test_a_row_s_routes_are_the_same_bits_in_calls_of_any_size(gpu, experts, top_k, groups, kept, scores, renormalize, biased):
+    """The weights in fp32 too, on both sides of where fewer lanes take a row, and of rows that 64 bits decide."""
+    r = np.random.default_rng(experts + top_k)
+    logits = np.concatenate([r.normal(0, 1.5, (150, experts)), 0.5 + r.integers(-9, 10, (20, experts)) * 2.0 ** -21, r.normal(0, 40, (10, experts))])
+    logits[20:30, r.permutation(experts)[:experts // 3]] = -np.inf
+    logits[30, 1:], logits[31] = np.nan, -np.inf
+    bias = r.normal(0, 0.05, experts) if biased else None
+    for logits_type in (F32, F16, BF16):
+        for best in (1, 2) if groups > 1 else (1,):
+            d = ref.desc(experts, top_k, scores, groups, kept, best, renormalize, 2.5)
+            idx, w = call(d, logits, bias, logits_type, weights_type=F32)
+            for rows in (1, 8191, 8192, 9001):
+                order = (np.arange(rows) * 7 + 3) % len(logits)
+                i2, w2 = call(d, logits[order], bias, logits_type, weights_type=F32)
+                assert np.array_equal(i2, idx[order])
+                bad = (w2.view(np.uint32) != w[order].view(np.uint32)).any(1)
+                assert not bad.any(), f"{rows} rows: {bad.sum()} differ, row {order[np.argmax(bad)]}: {w2[np.argmax(bad)]} and {w[order][np.argmax(bad)]}"
