@@ -526,13 +526,12 @@ __global__ __launch_bounds__(256) void k_route_rows_fast(RouteArgs a) {
         if constexpr (kSlots == 2) sum += lanes_sum<LANES>(w[1]);
         // (scores that fp32 does not hold well are 64 bits' again; none in service leaves zeros)
         if (a.sigmoid) certain &= sum > 1e-30f || lanes_max<LANES>(served[0] || served[kSlots - 1] ? 1u : 0u) == 0u;
-        const float factor = sum > 0.0f ? a.scaling / sum : 0.0f;
+        const float of_sum = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
-        for (uint32_t i = 0; i < kSlots; ++i) w[i] *= factor;
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < kSlots; ++i) w[i] *= a.scaling;
+        for (int i = 0; i < kSlots; ++i) w[i] *= of_sum;  // (first: the scaling over a small sum may leave fp32)
     }
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) w[i] *= a.scaling;
     if (real && certain)
 #pragma unroll
         for (uint32_t i = 0; i < kSlots; ++i)

@@ -148,3 +148,19 @@ def test_a_row_s_routes_are_the_same_bits_in_calls_of_any_size(gpu, experts, top
                 assert np.array_equal(i2, idx[order])
                 bad = (w2.view(np.uint32) != w[order].view(np.uint32)).any(1)
                 assert not bad.any(), f"{rows} rows: {bad.sum()} differ, row {order[np.argmax(bad)]}: {w2[np.argmax(bad)]} and {w[order][np.argmax(bad)]}"
+
+
+@pytest.mark.parametrize("scaling", [3e38, 1e30, 1e10, -1e30, 1e-30, 1e-38])
+@pytest.mark.parametrize("rows", [11, 8200])
+def test_any_finite_scaling_over_small_sums(gpu, scaling, rows):
+    """Chosen sigmoids that sum to 1e-3 ... 1e-29: the scaling over their sum alone may leave fp32, the weights do not."""
+    r = np.random.default_rng(11)
+    for experts, top_k in ((64, 8), (200, 20)):
+        logits = single(r.normal(0, 1, (11, experts)) - np.linspace(5, 68, 11)[:, None])
+        d = ref.desc(experts, top_k, SIGMOID, scaling=scaling)
+        want, weights, bound = ref.route(d, logits)
+        order = np.arange(rows) % 11
+        idx, w = call(d, logits[order], weights_type=F32)
+        assert np.array_equal(idx, want[order])
+        assert np.isfinite(w).all()
+        ref.assert_weights(w, weights[order], bound[order], F32, f"{scaling}")
