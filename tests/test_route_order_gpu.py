@@ -164,3 +164,29 @@ def test_any_finite_scaling_over_small_sums(gpu, scaling, rows):
         assert np.array_equal(idx, want[order])
         assert np.isfinite(w).all()
         ref.assert_weights(w, weights[order], bound[order], F32, f"{scaling}")
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
+@pytest.mark.parametrize("rows", [7, 8200])
+def test_every_nan_is_out_of_service(gpu, kind, rows):
+    """Quiet and signalling ones, of either sign, in the logits and in the bias."""
+    r = np.random.default_rng(3)
+    nans = {F32: (0x7FC00000, 0xFFC00000, 0x7F800001, 0xFF800001, 0x7FFFFFFF), F16: (0x7E00, 0xFE00, 0x7C01, 0xFC01, 0x7FFF), BF16: (0x7FC0, 0xFFC0, 0x7F81, 0xFF81, 0x7FFF)}[kind]
+    t = np.uint32 if kind == F32 else np.uint16
+    for experts, groups, kept, best in ((64, 1, 1, 1), (256, 8, 4, 2), (256, 8, 4, 1), (1000, 1, 1, 1)):
+        for scores, biased in ((SOFTMAX, False), (SIGMOID, True), (SOFTMAX, True)):
+            bits = ref.encode(r.normal(0, 1.5, (7, experts)), kind).view(t).copy()
+            own = ref.encode(r.normal(0, 0.05, experts), kind).view(t).copy()
+            for row in range(7):
+                bits[row, r.permutation(experts)[:5 * (row + 1)]] = np.resize(np.array(nans, t), 5 * (row + 1))
+            own[r.permutation(experts)[:5]] = np.array(nans, t)
+            seen, b = (ref.decode(v.view(np.float32) if kind == F32 else v, kind) for v in (bits, own))
+            d = ref.desc(experts, 8, scores, groups, kept, best)
+            want, weights, bound = ref.route(d, seen, b if biased else None)
+            order = np.arange(rows) % 7
+            x, on = rt.dev(np.ascontiguousarray(bits[order])), rt.dev(own)
+            idx, w = rt.empty(rows * 32).fill(0xA5), rt.empty(rows * 32).fill(0xA5)
+            rt.route_rows(d, x, kind, experts, on if biased else None, kind, idx, w, F32, rows)
+            rt.synchronize()
+            assert np.array_equal(idx.download(np.uint32, rows * 8).reshape(rows, 8), want[order])
+            ref.assert_weights(w.download(np.float32, rows * 8).reshape(rows, 8), weights[order], bound[order], F32)
