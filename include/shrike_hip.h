@@ -645,7 +645,9 @@ typedef struct {
     float scaling;
 } shrike_route_desc;
 /* Routes of `rows` rows of logits (fp32, fp16 or bf16, SHRIKE_ELEM_*), logits_stride_elements apart, any address of their own size; d_bias:
- * [num_experts] of bias_dtype, or NULL. out_indices: u32[rows, top_k]; out_weights: [rows, top_k] of weights_dtype. They feed
+ * [num_experts] of bias_dtype, or NULL. out_indices: u32[rows, top_k]; out_weights: [rows, top_k] of weights_dtype; neither overlaps an input. The
+ * indices are those of the choices in 64 bits; the weights are formed in fp32 and rounded once, off by 2^-19 of themselves at most, and by 2^-22 more for
+ * every unit that the logits lie from 0 (sigmoid) or below the largest one that counts (softmax). They feed
  * shrike_hip_group_pairs and shrike_hip_moe_resolve_batch as the routers' outputs do (fp16 weights). `desc` is read at the call. A row's routes
  * depend on that row alone: indices and weights are the same bits whatever the other rows and their number. */
 int shrike_hip_route_rows(void *stream, const shrike_route_desc *desc, const void *d_logits, uint32_t logits_dtype, uint64_t logits_stride_elements,
@@ -658,7 +660,7 @@ int shrike_hip_route_rows(void *stream, const shrike_route_desc *desc, const voi
  * 64 (this library's own) or 128; k: a multiple of group_size up to SHRIKE_AFFINE4_MAX_K; n up to 2^24; rows up to 2^22. x: fp16 or bf16, rows at 16-byte
  * aligned addresses, x_stride_elements apart (at most 2^36); out: fp16, bf16 or fp32, rows out_stride_elements apart (what lies between them is left as it
  * is). The codes are never rounded: products of a group are summed and scaled in fp32 and the result is rounded once. A group's sums of x * code (up
- * to 15 a value) and of x have to be finite in fp32; a row of x with an infinity or a NaN has outputs that are not finite, and no other row's change. The
+ * to 15 a value) and of x have to stay below 2^127, and 8 * scale of symmetric weights too; a row of x with an infinity or a NaN has outputs that are not finite, and no other row's change. The
  * order of the sums depends on rows, n and k, so calls of other sizes may differ in last places; the same call gives the same bits. out overlaps
  * no input. */
 int shrike_hip_affine4_product(void *stream, const void *d_x, uint32_t x_dtype, uint64_t x_stride_elements, const shrike_projection *w,
