@@ -282,9 +282,10 @@ __device__ __forceinline__ uint4 affine4_load16(buffer_t b, uint32_t at, uint32_
 // Up to 8 R8 rows a workgroup of eight waves; `parts` of them share an output block's k, the others have blocks of their own. A wave's
 // block is 32 outputs, a lane's column of it one output. Codes and rows come through LDS, a unit of 256 k (four steps, a line of a row of codes)
 // ahead, the rows a part's in two places, the codes a wave's own in one: they go on into registers before the next are asked for. While a unit is
-// multiplied, the group sums of its rows are formed beside it, and the bias term of the unit before is added. A unit's loads have only the unit before to
-// hide behind, and the waves meet at every unit: of their time they wait 40 to 58 % there (300 rows of 4,096 x 2,048 40, 64 of 16,384 x 2,304 53, 8 of 5,120 x
-// 2,880 58), and the vector unit is busy 51, 40 and 32 %, the matrix unit 16, 9 and 8. Of a unit's and wave's some 300 instructions 144 take the codes apart, 16 multiply. (Two sets of sums, so that one chain is scaled while the
+// multiplied, the group sums of its rows are formed beside it, and the bias term of the unit before is added. What bounds it is waiting: a unit's loads have
+// only the unit before to hide behind, and the waves meet at every unit. Of their time they wait 40 to 58 % (300 rows of 4,096 x 2,048 40, 64 of 16,384 x
+// 2,304 53, 8 of 5,120 x 2,880 58); the vector unit is busy 51, 40 and 32 %, the matrix unit 16, 9 and 8. Of some 300 instructions a unit and wave 144 take
+// the codes apart and 16 multiply. (Two sets of sums, so that one chain is scaled while the
 // next is multiplied, took the registers of two waves and 3 us more of 22; two copies of the loop for the scales of two units no less time.)
 // 8 rows of 5,120 x 2,880: 8.7 us; 37 of 2,049 x 2,304: 10.4; 64 of 16,384 x 2,304: 23.2 (0.86 TB/s of weights, 208 TFLOP/s).
 //
@@ -576,8 +577,8 @@ static int launch_few(const Affine4Args &args, hipStream_t s) {
 // tile's rows each. A wave takes a code apart for MT blocks of rows, and scales a chain while the next is multiplied.
 //
 // What bounds it is the issue of instructions beside the matrix ones: a step of a wave of 128 x 64 has 32 of these, 1,024 cycles, and some 390 of the vector
-// unit, half of them the scaling; the vector unit is busy 54 % of the time and the matrix unit 39. 4,096 rows of 8,192 x 4,096: 322 to 338 us by the card, 815 to 855 TFLOP/s (a large fp16 product of the library, whose weights are not taken
-// apart, 227); 512 of 8,192 x 2,048: 34 us. Without the loads the large one takes 12 % less, without the group sums 10 to 15. In two parts of k a CU
+// unit, half of them the scaling; the vector unit is busy 54 % of the time and the matrix unit 39. 4,096 rows of 8,192 x 4,096:
+// 322 to 338 us by the card, 815 to 855 TFLOP/s (a large fp16 product of the library, whose weights are not taken apart, 227); 512 of 8,192 x 2,048: 34 us. Without the loads the large one takes 12 % less, without the group sums 10 to 15. In two parts of k a CU
 // with one small tile has two waves a SIMD: 512 of 8,192 x 2,048 39 us against 44.
 
 // Four bytes a lane into LDS, as lds_load16

@@ -191,8 +191,8 @@ __global__ __launch_bounds__(256) void k_route_rows(RouteArgs a) {
 // a row has: its weights are the same bits in a call of any size.
 //
 // LANES lanes have a row, each up to NPL neighbouring experts of one group: 64 for few rows, which takes the fewest steps, 16 for many, where four rows
-// share every step between lanes. A step of the selection is the largest of a lane's words below the last one taken, and then of the row's lanes. The vector unit bounds it, busy
-// 99 % of the time: 16,384 rows of 512, top 10, take 21 us where their bytes take 7 (in 64 bits alone 75; every close row again in 64 bits 33; words with a test of range each 30). One row takes 3.2 us on the GPU, and
+// share every step between lanes. A step of the selection is the largest of a lane's words below the last one taken, and then of the row's lanes. The
+// vector unit bounds it, busy 99 % of the time: 16,384 rows of 512, top 10, take 21 us where their bytes take 7 (in 64 bits alone 75; every close row again in 64 bits 33; words with a test of range each 30). One row takes 3.2 us on the GPU, and
 // a call from the host 8.
 
 enum class RouteWord { kValue, kLogit, kLogit16 };
